@@ -54,6 +54,8 @@ SIGNATURES = {
     "hils_decode_step_paged_workspace_bytes": (_SZ, [_I] * 9),
     "hils_norm_rope_fwd": (_I, [_P] * 6 + [_I] * 5 + [_F, _I, _I, _P]),
     "hils_norm_rope_bwd": (_I, [_P] * 8 + [_I] * 7 + [_P]),
+    "hils_copy_pages": (_I, [_P] * 4 + [_I] * 3 + [_I64] * 2 + [_P]),
+    "hils_commit_drafts": (_I, [_P] * 5 + [_I] * 2 + [_P] * 2 + [_I] * 6 + [_I64, _I, _P]),
 }
 
 # kernels each entry point launches (memsets excluded); used to report launch counts

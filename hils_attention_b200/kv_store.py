@@ -14,24 +14,33 @@ a page boundary.  Inside a page the rows of one head are contiguous, (h_kv, 64, 
 is a single 16 KB run (D = 128) where the token-major layout has 64 rows h_kv * D apart.  The pooled chunk keys and their prior bias - one row per completed chunk, 1/64 of the
 store - are kept dense per sequence slot, since the selection streams all of them on every step.
 
+Full pages are never written again, so several sequences may share them: `fork` gives a second sequence the pages of the
+first (a reference count per page, only the unfinished last page is copied), `compact` moves the pages in use to the front of
+the pool.
+
 Host-side bookkeeping (free list, tables, lengths) is plain Python and mirrors what sits on the device;
 nothing here reads device memory back, so a decode step issues no synchronisation.
 """
 from __future__ import annotations
 
+from collections import Counter
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 
+from . import ops
+
 
 class PagePool:
-    """Free list of page ids.  Page 0 is reserved as the scratch page that inactive batch rows write to."""
+    """Free list of page ids and the number of sequences that hold each page.  Page 0 is reserved as the scratch page that
+    inactive batch rows write to."""
 
     def __init__(self, num_pages: int):
         if num_pages < 2:
             raise ValueError("a pool needs at least two pages (page 0 is the scratch page)")
         self.num_pages = int(num_pages)
         self._free: List[int] = list(range(self.num_pages - 1, 0, -1))   # pop() hands out 1, 2, 3, ...
+        self._refs: List[int] = [0] * self.num_pages
 
     @property
     def free(self) -> int:
@@ -46,13 +55,46 @@ class PagePool:
     def take(self, n: int = 1) -> List[int]:
         if n > len(self._free):
             raise MemoryError(f"paged store: {n} pages wanted, {len(self._free)} free of {self.num_pages - 1}")
-        return [self._free.pop() for _ in range(n)]
+        out = [self._free.pop() for _ in range(n)]
+        for p in out:
+            self._refs[p] = 1
+        return out
+
+    def share(self, pages: Sequence[int]) -> None:
+        """One more sequence holds each of `pages`."""
+        for p in pages:
+            if not 0 < p < self.num_pages or self._refs[p] == 0:
+                raise ValueError(f"page id {p} is not a page in use")
+        for p in pages:
+            self._refs[p] += 1
+
+    def shared(self, page: int) -> bool:
+        return self._refs[page] > 1
 
     def give(self, pages: Sequence[int]) -> None:
-        for p in pages:
+        """One sequence less holds each of `pages`; those nobody holds any more go back to the free list."""
+        pages = list(pages)
+        for p, n in Counter(pages).items():
             if not 0 < p < self.num_pages:
                 raise ValueError(f"page id {p} is not a pool page")
-        self._free.extend(reversed(list(pages)))
+            if self._refs[p] < n:
+                raise ValueError(f"page id {p} is already free")
+        for p in reversed(pages):
+            self._refs[p] -= 1
+            if self._refs[p] == 0:
+                self._free.append(p)
+
+    def compact(self) -> Tuple[List[int], List[int]]:
+        """Renumber the pages in use to 1 .. n (n pages in use): returns the moved pages' old and new ids and rebuilds the
+        free list.  The contents are the caller's to copy."""
+        used = [p for p in range(1, self.num_pages) if self._refs[p]]
+        n = len(used)
+        src = [p for p in used if p > n]
+        dst = [p for p in range(1, n + 1) if not self._refs[p]]
+        for a, b in zip(src, dst):
+            self._refs[a], self._refs[b] = 0, self._refs[a]
+        self._free = list(range(self.num_pages - 1, n, -1))
+        return src, dst
 
 
 class PagedKVStore:
@@ -154,6 +196,55 @@ class PagedKVStore:
         self.lens[slot:slot + 1].zero_()
         self._active_dev[slot:slot + 1].zero_()
 
+    def fork(self, slot: int, copies: int = 1) -> List[int]:
+        """Start `copies` further sequences with the contents of `slot` (parallel samples, beams, a shared prompt); returns
+        their slots.  Full pages are shared, the unfinished last page and the pooled chunk keys are copied."""
+        if self._in_step:
+            raise RuntimeError("fork() between begin_step() and end_step()")
+        if not self._active[slot]:
+            raise ValueError(f"slot {slot} is not active")
+        if copies < 0:
+            raise ValueError(f"{copies} copies")
+        free = [b for b in range(self.max_seqs) if not self._active[b]][:copies]
+        if len(free) < copies:
+            raise MemoryError(f"paged store: {copies} sequence slots wanted, {len(free)} free")
+        T = self._lens[slot]
+        full, rem = T // self.S, T % self.S
+        head = self._tables[slot][:full]
+        new = self.pool.take(copies if rem else 0)
+        if rem and new:
+            self._copy_pages([self._tables[slot][full]] * copies, new)
+        for i, b in enumerate(free):
+            self.pool.share(head)
+            self._tables[b] = head + new[i:i + 1]
+            self._lens[b], self._active[b] = T, True
+            self._set_table(b, 0, self._tables[b])
+            self.lens[b:b + 1].fill_(T)
+            self._active_dev[b:b + 1].fill_(1)
+            if full:
+                self.lmk_k[:, b, :full].copy_(self.lmk_k[:, slot, :full])
+                self.prior_b[:, b, :full].copy_(self.prior_b[:, slot, :full])
+        return free
+
+    def compact(self) -> int:
+        """Move the pages in use to the front of the pool (ids 1 .. pages in use): what lies behind is free, and a snapshot of
+        the cache is one slice.  Returns the number of pages moved."""
+        if self._in_step:
+            raise RuntimeError("compact() between begin_step() and end_step()")
+        src, dst = self.pool.compact()
+        if src:
+            self._copy_pages(src, dst)
+            to = dict(zip(src, dst))
+            for b in self.active_slots():
+                table = [to.get(p, p) for p in self._tables[b]]
+                if table != self._tables[b]:
+                    self._tables[b] = table
+                    self._set_table(b, 0, table)
+        return len(src)
+
+    def _copy_pages(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        ops.copy_pages(self.k_pages, self.v_pages, src, dst)
+
     # ---- contents ------------------------------------------------------------------------------------
     def write_prefill(self, slot: int, layer: int, k: torch.Tensor, v: torch.Tensor, lmk_k: Optional[torch.Tensor] = None,
                       prior_b: Optional[torch.Tensor] = None) -> None:
@@ -163,6 +254,8 @@ class PagedKVStore:
         if k.shape != (T, self.h_kv, self.D) or v.shape != k.shape:
             raise ValueError(f"write_prefill: expected ({T}, {self.h_kv}, {self.D}), got {tuple(k.shape)} / {tuple(v.shape)}")
         pages = self._tables[slot]
+        if any(self.pool.shared(p) for p in pages):
+            raise RuntimeError(f"write_prefill: slot {slot} shares pages with another sequence")
         full, rem = T // self.S, T % self.S
         if full:
             ids = torch.tensor(pages[:full], dtype=torch.long, device=self.device)
@@ -195,20 +288,26 @@ class PagedKVStore:
         takes a page) and return max_len, the host-side bound of the lengths that the step call wants."""
         if self._in_step:
             raise RuntimeError("begin_step() twice without end_step()")
-        need = [b for b in range(self.max_seqs) if self._active[b] and self._lens[b] % self.S == 0]
-        for b in need:
-            if len(self._tables[b]) >= self.max_pages:
-                raise MemoryError(f"paged store: the sequence in slot {b} has reached {self.max_pages} pages")
-        if len(need) > self.pool.free:
-            raise MemoryError(f"paged store: {len(need)} pages wanted, {self.pool.free} free")
-        for b in need:
-            c = self._lens[b] // self.S
-            if len(self._tables[b]) == c:          # the page of position lens[b] may already be reserved
-                pg = self.pool.take(1)
-                self._tables[b].extend(pg)
-                self._set_table(b, c, pg)
+        self._reserve({b: 1 for b in self.active_slots()})
         self._in_step = True
         return max((self._lens[b] for b in range(self.max_seqs) if self._active[b]), default=0)
+
+    def _reserve(self, more) -> None:
+        """Take the pages that more[b] further tokens of the sequence in slot b need beyond those its table holds (some may
+        already be reserved); all or nothing."""
+        need = {b: (self._lens[b] + n + self.S - 1) // self.S for b, n in more.items()}
+        for b, c in need.items():
+            if c > self.max_pages:
+                raise MemoryError(f"paged store: the sequence in slot {b} has reached {self.max_pages} pages")
+        want = sum(max(0, c - len(self._tables[b])) for b, c in need.items())
+        if want > self.pool.free:
+            raise MemoryError(f"paged store: {want} pages wanted, {self.pool.free} free")
+        for b, c in need.items():
+            have = len(self._tables[b])
+            if c > have:
+                pg = self.pool.take(c - have)
+                self._tables[b].extend(pg)
+                self._set_table(b, have, pg)
 
     def step_args(self, layer: int):
         """(k_pages, v_pages, page_table, lens, lmk_k, prior_b) of one layer for the current batch."""

@@ -510,6 +510,91 @@ def decode_step_paged(q, lmk_q, k_new, v_new, k_pages, v_pages, page_table, lens
 
 
 # ------------------------------------------------------------------------------------------
+# pages of the paged store
+# ------------------------------------------------------------------------------------------
+def _host_ids(x, what: str) -> torch.Tensor:
+    """A sequence of ints or an integer CPU tensor as a contiguous int32 CPU tensor."""
+    if isinstance(x, torch.Tensor):
+        if x.is_cuda:
+            raise ValueError(f"{what} are host data (a sequence of ints or a CPU tensor), got a tensor on {x.device}")
+        if x.dtype == torch.int32:
+            t = x
+        elif x.dtype == torch.int64:
+            t = x.to(torch.int32)
+            if not torch.equal(t.to(torch.int64), x):
+                raise ValueError(f"{what} do not fit 32 bits")
+        else:
+            raise TypeError(f"{what} must be int32 or int64, got {x.dtype}")
+        if t.dim() != 1:
+            raise ValueError(f"{what} must be one-dimensional, got shape {tuple(x.shape)}")
+        return t.contiguous()
+    return torch.tensor(list(x), dtype=torch.int32)
+
+
+def _pool_layers(k_pages, v_pages, what: str):
+    """(layers, pages per layer, bytes from layer to layer) of two pools (num_layers, num_pages, h_kv, S, D) or one layer of them."""
+    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.stride() != v_pages.stride():
+        raise ValueError(f"{what}: k_pages and v_pages differ in shape, type or strides")
+    if k_pages.dim() not in (4, 5):
+        raise ValueError(f"{what}: pools are (num_pages, h_kv, S, D) or (num_layers, num_pages, h_kv, S, D), got {tuple(k_pages.shape)}")
+    layers = k_pages.shape[0] if k_pages.dim() == 5 else 1
+    first = k_pages[0] if k_pages.dim() == 5 else k_pages
+    if not first.is_contiguous():
+        raise ValueError(f"{what}: a layer's pool must be contiguous")
+    step = k_pages.stride(0) if k_pages.dim() == 5 else first.numel()
+    return layers, first.shape[0], step * k_pages.element_size()
+
+
+def copy_pages(k_pages, v_pages, src, dst) -> None:
+    """Copy pages src[i] -> dst[i] of a paged store, K and V, in all layers, in place.
+
+    k_pages, v_pages (num_layers, num_pages, h_kv, S, D) or one layer of them; src, dst page ids on the HOST (sequences of
+    ints or CPU tensors) of equal length.  A page may be copied to several others; an id outside the pool, a page written
+    twice and a page that is both read and written are refused (the copies run in no order).  A captured graph replays the
+    ids it was captured with."""
+    layers, pages, layer_bytes = _pool_layers(k_pages, v_pages, "copy_pages")
+    s, d = _host_ids(src, "page ids"), _host_ids(dst, "page ids")
+    if s.numel() != d.numel():
+        raise ValueError(f"copy_pages: {s.numel()} source and {d.numel()} destination pages")
+    if layers == 0 or s.numel() == 0:
+        return
+    page_bytes = k_pages.shape[-3] * k_pages.shape[-2] * k_pages.shape[-1] * k_pages.element_size()
+    call("hils_copy_pages", ptr(k_pages), ptr(v_pages), s.data_ptr(), d.data_ptr(), s.numel(), layers, pages, layer_bytes, page_bytes,
+         stream())
+
+
+def commit_drafts(k_draft, v_draft, k_pages, v_pages, page_table, lens, path) -> None:
+    """Write the accepted path of a drafted tree into the pages of its sequence, K and V, in all layers, in place.
+
+    k_draft, v_draft (num_layers, B, n, h_kv, D) or (B, n, h_kv, D) for one layer: the drafted tokens; k_pages, v_pages the
+    pools, (num_layers, num_pages, h_kv, 64, D) or one layer; page_table (B, max_pages) and lens (B) int32 as in
+    decode_step_paged; path (B, m <= n) int32 on the device: the nodes to keep, in order, up to the first negative entry.
+    Node path[b, i] becomes token lens[b] + i; lens is left as it is, no other row is touched."""
+    layers, pages, layer_bytes = _pool_layers(k_pages, v_pages, "commit_drafts")
+    one = k_pages.dim() == 4
+    if k_draft.shape != v_draft.shape or k_draft.dim() != (4 if one else 5):
+        raise ValueError(f"commit_drafts: drafts {tuple(k_draft.shape)} / {tuple(v_draft.shape)} for pools {tuple(k_pages.shape)}")
+    B, n, h_kv, D = k_draft.shape[-4:]
+    if (not one and k_draft.shape[0] != layers) or k_pages.shape[-3:] != (h_kv, 64, D):
+        raise ValueError(f"commit_drafts: drafts {tuple(k_draft.shape)} do not fit pools {tuple(k_pages.shape)}")
+    if k_draft.dtype != k_pages.dtype or v_draft.dtype != k_pages.dtype:
+        raise TypeError(f"commit_drafts: drafts of {k_draft.dtype} / {v_draft.dtype}, pools of {k_pages.dtype}")
+    for name, t in (("page_table", page_table), ("lens", lens), ("path", path)):
+        if t.dtype != torch.int32:
+            raise TypeError(f"commit_drafts: {name} must be int32, got {t.dtype}")
+    if page_table.dim() != 2 or path.dim() != 2 or page_table.shape[0] != B or lens.shape != (B,) or path.shape[0] != B or path.shape[1] > n:
+        raise ValueError(f"commit_drafts: page_table {tuple(page_table.shape)}, lens {tuple(lens.shape)}, path {tuple(path.shape)} for "
+                         f"{B} sequences of {n} nodes")
+    for t in (k_draft, v_draft, page_table, lens, path):
+        if not t.is_contiguous():
+            raise ValueError("commit_drafts: drafts, page_table, lens and path must be contiguous")
+    if B == 0 or layers == 0 or path.shape[1] == 0:
+        return
+    call("hils_commit_drafts", ptr(k_draft), ptr(v_draft), ptr(k_pages), ptr(v_pages), ptr(page_table), page_table.shape[1], pages, ptr(lens),
+         ptr(path), layers, B, n, path.shape[1], h_kv, D, layer_bytes, dtype_code(k_pages), stream())
+
+
+# ------------------------------------------------------------------------------------------
 # per-head RMSNorm + rotary embedding
 # ------------------------------------------------------------------------------------------
 class _NormRope(torch.autograd.Function):

@@ -312,6 +312,28 @@ int hils_norm_rope_bwd(const void* x, const void* weight, const void* cos, const
                        const float* rstd, const void* d_out, void* d_x, float* d_weight,
                        int B, int L, int H, int D, int cos_batched, int dtype, int cs_dtype, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Pages of the paged store moved on the device (fork of a sequence, compaction of the pool, acceptance of drafted
+ * tokens).  No counterpart in the reference, whose cache layer copies whole caches (utils/hils_cache_utils.py:45-62).
+ *
+ * hils_copy_pages: page src[i] -> page dst[i] for every i < n_pairs, in n_layers layers of both pools, one launch per 480
+ *   pairs.  src and dst are HOST arrays: they travel with the launch (a captured graph replays the ids of the capture).
+ *   Layer l of a pool starts l * layer_bytes behind its first; a page is page_bytes (a multiple of 16) long.  A page may be
+ *   read several times; one that is written twice, or read and written, by one call is refused, as is an id outside
+ *   [0, num_pages).
+ * hils_commit_drafts: the accepted path of a drafted tree goes into the pages of its sequence.  k_draft, v_draft (n_layers,
+ *   B, n, h_kv, D) hold the drafted tokens; path (B, m) int32, device, m <= n: the nodes to keep, in order, up to the first
+ *   negative entry; node path[b][i] becomes token lens[b] + i, row (lens[b] + i) % 64 of page
+ *   page_table[b][(lens[b] + i) / 64], (num_pages, h_kv, 64, D) per layer, layers layer_bytes apart.  lens is NOT advanced,
+ *   no other row is touched.  A path entry that is no node ends the path (hils_take_device_status: 8100001), a page
+ *   outside the pool or the table is skipped (8100002).
+ * ------------------------------------------------------------------------------------- */
+int hils_copy_pages(void* k_pages, void* v_pages, const int32_t* src, const int32_t* dst, int n_pairs, int n_layers,
+                    int num_pages, int64_t layer_bytes, int64_t page_bytes, void* stream);
+int hils_commit_drafts(const void* k_draft, const void* v_draft, void* k_pages, void* v_pages, const int32_t* page_table,
+                       int page_stride, int num_pages, const int32_t* lens, const int32_t* path, int n_layers, int B,
+                       int n, int m, int h_kv, int D, int64_t layer_bytes, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
