@@ -54,9 +54,19 @@ SIGNATURES = {
     "hils_decode_step_paged_workspace_bytes": (_SZ, [_I] * 9),
     "hils_norm_rope_fwd": (_I, [_P] * 6 + [_I] * 5 + [_F, _I, _I, _P]),
     "hils_norm_rope_bwd": (_I, [_P] * 8 + [_I] * 7 + [_P]),
+    "hils_qk_norm_rope_fwd": (_I, [_P, _I, _P, _I, _I64, _I64, _P] + [_I] * 5 + [_F] * 2 + [_I] * 2 + [_P]),
+    "hils_qk_norm_rope_bwd": (_I, [_P, _I, _P, _I, _I64, _I64, _P] + [_I] * 5 + [_F] * 2 + [_I] * 2 + [_P, _SZ, _P]),
+    "hils_qk_norm_rope_bwd_workspace_bytes": (_SZ, [_I]),
     "hils_copy_pages": (_I, [_P] * 4 + [_I] * 3 + [_I64] * 2 + [_P]),
     "hils_commit_drafts": (_I, [_P] * 5 + [_I] * 2 + [_P] * 2 + [_I] * 6 + [_I64, _I, _P]),
 }
+
+class RopeTensor(C.Structure):
+    """hils_rope_tensor of the header."""
+    _fields_ = ([(n, _P) for n in ("x", "weight", "out", "d_out", "d_weight")] +
+                [(n, _I64) for n in ("x_stride_b", "x_stride_l", "x_stride_h", "g_stride_b", "g_stride_l", "g_stride_h")] +
+                [("heads", C.c_int32), ("reserved", C.c_int32)])
+
 
 # kernels each entry point launches (memsets excluded); used to report launch counts
 KERNELS_PER_CALL = {
@@ -64,7 +74,7 @@ KERNELS_PER_CALL = {
     "hils_topk_fwd": 1, "hils_topk_bwd": 2, "hils_topk_bwd_noalloc": 2, "hils_sparse_attn_fwd": 6, "hils_sparse_attn_bwd": 6, "hils_sparse_attn_bwd_with_index": 6,
     "hils_chunk_logz_fwd": 1, "hils_chunk_logz_bwd": 2, "hils_swa_fwd": 1, "hils_swa_bwd": 2,
     "hils_chunk_weights_fwd": 1, "hils_chunk_weights_bwd": 1, "hils_combine_fwd": 1, "hils_combine_bwd": 1,
-    "hils_norm_rope_fwd": 1, "hils_norm_rope_bwd": 1,
+    "hils_norm_rope_fwd": 1, "hils_norm_rope_bwd": 1, "hils_qk_norm_rope_fwd": 1, "hils_qk_norm_rope_bwd": 2,
     "hils_decode_step_paged": 5,   # append, then as below
     "hils_decode_step": 4,   # window, key stream, selection + inter-chunk softmax, sparse + combine (the 2 copies not counted)
 }

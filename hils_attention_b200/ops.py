@@ -19,9 +19,10 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, dtype_code, ptr, query, stream
+from ._lib import F32, call, dtype_code, ptr, query, stream
 
 __all__ = [
     "chunk_attn_pool", "chunk_attn_pool_tilelang", "chunk_mean_pool", "online_softmax_topk_head",
@@ -661,6 +662,141 @@ def single_tensor_rope_autograd(x, x_cos, x_sin):
 def rope_rotary_pos_emb(q, k, cos, sin):
     """Rotary embedding of q and k (ops/rope_tilelang_fp32.py:84-88): returns (q_out, k_out)."""
     return _NormRope.apply(q, None, cos, sin, 0.0), _NormRope.apply(k, None, cos, sin, 0.0)
+
+
+def rope_frequencies(rot: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
+                     original_length: int = 8192, beta_fast: float = 32.0, beta_slow: float = 1.0, device=None):
+    """Inverse frequencies of a rotary embedding over `rot` elements and the factor its cos and sin are multiplied by:
+    (inv_freq (rot/2) float64, attention_scaling), the arguments of `qk_norm_rope`.
+
+    inv_freq[i] = base ** (-2i / rot).  For contexts `factor` times longer than the `original_length` a model was trained on:
+    scaling="linear" divides every frequency by factor; "ntk" stretches the base by factor ** (rot / (rot - 2)), which
+    leaves the fastest pair as it is and divides the slowest by factor; "yarn" keeps the pairs that turn more than
+    beta_fast times over original_length, divides those that turn less than beta_slow times, blends linearly between, and
+    scales by 1 + ln(factor) / 10."""
+    if rot < 0 or rot % 2:
+        raise ValueError(f"rope_frequencies: the rotated part must be even, got {rot}")
+    if base <= 1.0 or factor < 1.0:
+        raise ValueError(f"rope_frequencies: base {base} and factor {factor} must be larger than 1 and at least 1")
+    i = torch.arange(0, rot, 2, dtype=torch.float64)
+    scale = 1.0
+    if scaling == "ntk":
+        if rot < 4:
+            raise ValueError("rope_frequencies: scaling='ntk' needs rot >= 4")
+        base = base * factor ** (rot / (rot - 2))
+    inv = base ** (-i / max(rot, 1))
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "yarn":
+        def pair_that_turns(n):        # index of the pair that makes n turns over the original length
+            return rot * math.log(original_length / (n * 2 * math.pi)) / (2 * math.log(base))
+        low = max(math.floor(pair_that_turns(beta_fast)), 0)
+        high = min(math.ceil(pair_that_turns(beta_slow)), rot - 1)
+        slow = ((i / 2 - low) / max(high - low, 1e-3)).clamp(0, 1)
+        inv = inv * (1 - slow) + inv / factor * slow
+        scale = 1.0 + 0.1 * math.log(factor)
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"rope_frequencies: scaling {scaling!r} is none of None, 'linear', 'ntk', 'yarn'")
+    return inv.to(device) if device is not None else inv, scale
+
+
+def _rope_rows(x):
+    """x (B,L,H,D) as the kernel reads it: any strides over a dense last dimension, first element on a 16-byte boundary."""
+    if x.stride(-1) != 1 and x.shape[-1] > 1 or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x
+
+
+def _rope_call(name, sides, pos, inv_freq, interleaved, scaling, eps, w_dtype, ws=None):
+    """sides: (x or None, weight, out, d_out, d_weight) of each tensor."""
+    B, L, _, D = sides[0][2].shape
+    t = (_lib.RopeTensor * len(sides))()
+    for r, (x, w, out, g, dw) in zip(t, sides):
+        r.x, r.weight, r.out, r.d_out, r.d_weight = ptr(x), ptr(w), ptr(out), ptr(g), ptr(dw)
+        if x is not None:
+            r.x_stride_b, r.x_stride_l, r.x_stride_h = x.stride()[:3]
+        if g is not None:
+            r.g_stride_b, r.g_stride_l, r.g_stride_h = g.stride()[:3]
+        r.heads = out.shape[2]
+    ps = pos.stride() if pos.dim() == 2 else (0, pos.stride(0))
+    args = [t, len(sides), ptr(pos) if pos.numel() else None, int(pos.dtype == torch.int64), 0 if pos.dim() == 2 and pos.shape[0] == 1 else ps[0],
+            ps[1], ptr(inv_freq), 2 * inv_freq.numel(), B, L, D, int(interleaved), scaling, eps, dtype_code(sides[0][2]), w_dtype]
+    if ws is not None:
+        args += [ptr(ws), ws.numel()]
+    call(name, *args, stream())
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, interleaved, scaling, eps):
+        xs = [_rope_rows(x) for x in (q, k) if x is not None]
+        ws = [w for x, w in ((q, q_weight), (k, k_weight)) if x is not None]
+        outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+        w_dtype = next((dtype_code(w) for w in ws if w is not None), F32)
+        _rope_call("hils_qk_norm_rope_fwd", [(x, w, o, None, None) for x, w, o in zip(xs, ws, outs)], positions, inv_freq, interleaved, scaling,
+                   eps, w_dtype)
+        # without a norm the backward is the rotation back, which does not read x
+        ctx.save_for_backward(positions, inv_freq, *[t for x, w in zip(xs, ws) if w is not None for t in (x, w)])
+        ctx.meta = ([w is not None for w in ws], [(x.shape, x.dtype) for x in xs], interleaved, scaling, eps, w_dtype)
+        return outs[0], (outs[1] if k is not None else None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_q, d_k):
+        weighted, like, interleaved, scaling, eps, w_dtype = ctx.meta
+        positions, inv_freq, *saved = ctx.saved_tensors
+        given = iter(saved)
+        grads, d_ws, sides = [None, None], [None, None], []
+        for i, (has, (shape, dtype), g) in enumerate(zip(weighted, like, (d_q, d_k))):
+            x, w = (next(given), next(given)) if has else (None, None)
+            if not (ctx.needs_input_grad[i] or ctx.needs_input_grad[2 + i]):
+                continue
+            grads[i] = torch.empty(shape, dtype=dtype, device=positions.device)
+            d_ws[i] = None if w is None else torch.empty_like(w)
+            sides.append((x, w, grads[i], _rope_rows(g.to(dtype)), d_ws[i]))
+        if sides:
+            ws_bytes = query("hils_qk_norm_rope_bwd_workspace_bytes", like[0][0][-1]) if any(weighted) else 0
+            tmp = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=positions.device)
+            _rope_call("hils_qk_norm_rope_bwd", sides, positions, inv_freq, interleaved, scaling, eps, w_dtype, tmp)
+        return (*grads, *d_ws, None, None, None, None, None)
+
+
+def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: float = 1e-6, interleaved: bool = False,
+                 attention_scaling: float = 1.0):
+    """Per-head RMSNorm of queries and keys and the rotation of their positions, in one pass over both tensors.
+
+    q (B,L,h_q,D), k (B,L,h_k,D) or None, bf16 or fp32, D even and at most 256; slices of a fused projection are read in
+    place.  positions (L,), (1,L) or (B,L) int32 or int64: any position for any token (ragged decode batches, drafted trees),
+    so no cos/sin table is gathered.  inv_freq (rot/2) float64 or float32, radians per position (`rope_frequencies`);
+    rot <= D, the elements behind it are not rotated; pairs are (i, i + rot/2), interleaved (2i, 2i + 1).  q_weight, k_weight
+    (D,) or None (no norm for that tensor).  Arithmetic in fp32 with one rounding.  Returns (q_out, k_out or None), dense;
+    differentiable with respect to q, k and the weights (once)."""
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+        raise ValueError(f"qk_norm_rope: q (B,L,h_q,D) and k (B,L,h_k,D), got {tuple(q.shape)} and {None if k is None else tuple(k.shape)}")
+    B, L, _, D = q.shape
+    dtype_code(q)
+    if k is not None and k.dtype != q.dtype:
+        raise TypeError(f"qk_norm_rope: q of {q.dtype}, k of {k.dtype}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"qk_norm_rope: positions must be int32 or int64, got {positions.dtype}")
+    if positions.shape not in ((L,), (1, L), (B, L)):
+        raise ValueError(f"qk_norm_rope: positions {tuple(positions.shape)} for {B} x {L} tokens")
+    if inv_freq.dim() != 1 or inv_freq.dtype not in (torch.float32, torch.float64) or 2 * inv_freq.shape[0] > D:
+        raise ValueError(f"qk_norm_rope: inv_freq must be (at most {D // 2},) float64 or float32, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
+    weights = [w for w in (q_weight, k_weight if k is not None else None) if w is not None]
+    for w in weights:
+        if w.shape != (D,):
+            raise ValueError(f"qk_norm_rope: a weight of shape {tuple(w.shape)} for heads of {D}")
+    if len(weights) == 2 and weights[0].dtype != weights[1].dtype:
+        raise TypeError(f"qk_norm_rope: weights of {weights[0].dtype} and {weights[1].dtype}")
+    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    if inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous():
+        inv_freq = inv_freq.double().contiguous()
+    if positions.data_ptr() % 16:
+        positions = positions.clone()
+    return _QkNormRope.apply(q, k, q_weight, k_weight, positions, inv_freq, bool(interleaved), float(attention_scaling), float(eps))
 
 
 class _ExactChunkLogZ(torch.autograd.Function):

@@ -334,6 +334,39 @@ int hils_commit_drafts(const void* k_draft, const void* v_draft, void* k_pages, 
                        int page_stride, int num_pages, const int32_t* lens, const int32_t* path, int n_layers, int B,
                        int n, int m, int h_kv, int D, int64_t layer_bytes, int dtype, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Norm of queries and keys per head and the rotation of their positions, both tensors in one launch, from integer
+ * positions instead of cos/sin tables.  What hils_norm_rope_* does for one tensor and a table, in the form that ragged
+ * decode batches and drafted trees need (modeling_olmo_hils.py:105-111 chained with ops/rope_tilelang_fp32.py:96-181).
+ *   Element (b, l, h, d) of tensor i sits at x + (b*x_stride_b + l*x_stride_l + h*x_stride_h + d) elements (any strides: a
+ *   slice of a fused projection is read in place); out is dense (B, L, heads, D).  weight (D) in weight_dtype or NULL (no
+ *   norm).  positions: int32 or (positions_64 != 0) int64, element b*pos_stride_b + l*pos_stride_l.  inv_freq (rot/2)
+ *   fp64, device: radians per position; rot <= D even, elements from rot on are not rotated; interleaved: pairs
+ *   (2i, 2i+1), else (i, i + rot/2); cos and sin are multiplied by `scaling`.  D even, at most 256.  fp32 arithmetic, one
+ *   rounding.
+ *   Backward: d_out with its own strides, out = d_x (dense), d_weight (D) in weight_dtype, summed in a fixed order;
+ *   workspace: hils_qk_norm_rope_bwd_workspace_bytes() bytes when a weight is given.
+ * ------------------------------------------------------------------------------------- */
+typedef struct {
+  const void* x;
+  const void* weight;
+  void* out;
+  const void* d_out;
+  void* d_weight;
+  int64_t x_stride_b, x_stride_l, x_stride_h;
+  int64_t g_stride_b, g_stride_l, g_stride_h;
+  int32_t heads, reserved;
+} hils_rope_tensor;
+
+int hils_qk_norm_rope_fwd(const hils_rope_tensor* tensors, int n_tensors, const void* positions, int positions_64,
+                          int64_t pos_stride_b, int64_t pos_stride_l, const double* inv_freq, int rot, int B, int L, int D,
+                          int interleaved, float scaling, float eps, int dtype, int weight_dtype, void* stream);
+int hils_qk_norm_rope_bwd(const hils_rope_tensor* tensors, int n_tensors, const void* positions, int positions_64,
+                          int64_t pos_stride_b, int64_t pos_stride_l, const double* inv_freq, int rot, int B, int L, int D,
+                          int interleaved, float scaling, float eps, int dtype, int weight_dtype, void* workspace,
+                          size_t workspace_bytes, void* stream);
+size_t hils_qk_norm_rope_bwd_workspace_bytes(int D);
+
 #ifdef __cplusplus
 }
 #endif
