@@ -149,19 +149,25 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
         raise RuntimeError("hils_b200 kernels need CUDA tensors (no CPU fallback exists)")
     # The kernels read rows with 8- and 16-byte vector loads and through TMA descriptors: a tensor that starts inside
     # a 16-byte word (an odd slice of a larger buffer) would fault on the device, so it is refused here.
-    if t.data_ptr() % 16 != 0 and t.numel() * t.element_size() >= 16:
+    a = t.data_ptr()
+    if a & 15 and t.numel() * t.element_size() >= 16:
         _pending().clear()
         raise ValueError(f"hils_b200: tensor of shape {tuple(t.shape)} starts at an address that is not 16-byte aligned "
                          "(a view into the middle of a buffer?); copy it with .clone() first. Nothing was launched")
-    _pending().append(t.device)
-    return t.data_ptr()
+    try:
+        _tls.devs.append(t.device)
+    except AttributeError:                                     # this thread's first tensor
+        _pending().append(t.device)
+    return a
 
 
 def stream() -> int:
     """Current torch stream of the device the pending call's tensors live on (the kernels follow their
     tensors, like the reference's ops, not the process-wide current device)."""
     dev = _call_device()
-    return torch.cuda.current_stream(dev).cuda_stream
+    if dev is None:
+        return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev.index)       # the same handle without building a Stream object per call
 
 
 def call(name: str, *args):
@@ -171,7 +177,7 @@ def call(name: str, *args):
     lib = load()
     dev = _call_device()
     _pending().clear()
-    if dev is not None and torch.cuda.current_device() != dev.index:
+    if dev is not None and torch._C._cuda_getDevice() != dev.index:
         with torch.cuda.device(dev):
             rc = getattr(lib, name)(*args)
     else:

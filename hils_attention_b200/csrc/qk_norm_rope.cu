@@ -14,7 +14,11 @@
 //
 // Layout.  2V elements of a row (V pairs) are one unit, a lane owns one unit and a group of lanes (the next power of two of
 // the units) one row, so the row's sums are a few shuffles and a group reads and writes whole rows with 16-byte accesses.
-// A group forms the cos/sin of its token once and walks `hpg` heads with it, kHeads rows in flight.
+// A group forms the cos/sin of its token once and walks `hpg` heads with it, the rows of the next four steps on their way.
+//
+// What bounds it: the HBM.  Forward 2, backward 3 tensors' worth of bytes; 65536 tokens, 32 + 32 heads of 128, bf16: 348 us
+// = 6.16 TB/s and 580 us = 5.55 TB/s (0.94 and 0.85 of the copy bandwidth; the issue slots are 60 to 70 % busy).  With the
+// loads in registers, four rows at a time, it was 908 and 1682 us.
 #include <algorithm>
 
 #include "common.cuh"
@@ -52,9 +56,12 @@ __device__ __forceinline__ void load_v(const T* p, float (&f)[V]) {
       f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   } else {
-    static_assert(V == 4, "a unit half is 1, 4 or (bf16) 8 elements");
-    const float4 v = load4(p);
-    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    static_assert(V == 4 || V == 8, "a unit half is 1, 4 or 8 elements");
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 v = load4(p + i);
+      f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+    }
   }
 }
 
@@ -113,11 +120,37 @@ __device__ __forceinline__ float weight_at(const QkParams& p, const void* w, int
   return p.w_f32 ? static_cast<const float*>(w)[d] : to_f(static_cast<const bf16*>(w)[d]);
 }
 
+// Rows per lane on their way from global memory (asynchronous copies into slots that only their own thread reads, so they
+// need no barrier).  The kernel holds 80 (forward) or 128 (backward) registers of working values per thread; loads kept in
+// registers as well leave too few warps to cover the memory's latency.  Four steps ahead with two CTAs per SM measured best:
+// backward at 64K tokens 580 us, six ahead 697, three CTAs (which spill) 1854; the weights sit in shared memory, not in
+// registers, for the same reason (808 us with them in registers).
+template <typename T, int V>
+constexpr bool kQkAsync = V * sizeof(T) >= 8;
+constexpr int kQkStages = 4;
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
+}
+
+template <typename T, int V, int UPL, bool BWD>
+constexpr size_t qk_smem() {
+  const size_t ring = kQkAsync<T, V> ? (size_t)kQkStages * (BWD ? 4 : 2) * kQkThreads * V * sizeof(T) : 0;
+  const size_t dw = BWD ? (size_t)(kQkThreads / 32) * kQkMaxD * sizeof(float) : 0;
+  return (kQkMaxD / 2) * sizeof(unsigned long long) + kQkMaxD * sizeof(float) + (ring > dw ? ring : dw);
+}
+
 template <typename T, int V, int UPL, bool INTER, bool BWD>
-__global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const __grid_constant__ QkParams p) {
-  constexpr int kHeads = UPL > 1 ? 1 : (BWD ? 2 : 4);          // rows in flight per lane
-  __shared__ unsigned long long turn_s[kQkMaxD / 2];
-  __shared__ float dw_s[BWD ? kQkThreads / 32 : 1][BWD ? kQkMaxD : 1];
+__global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_kernel(const __grid_constant__ QkParams p) {
+  constexpr bool kAsync = kQkAsync<T, V>;
+  constexpr int kParts = BWD ? 4 : 2, kBytes = V * sizeof(T);
+  extern __shared__ __align__(16) unsigned char qk_smem_raw[];
+  unsigned long long* turn_s = reinterpret_cast<unsigned long long*>(qk_smem_raw);
+  float* w_s = reinterpret_cast<float*>(turn_s + kQkMaxD / 2);
+  unsigned char* ring = reinterpret_cast<unsigned char*>(w_s + kQkMaxD);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int si = (p.n_sides > 1 && (int)blockIdx.x >= p.side[1].cta0) ? 1 : 0;
   const QkSide& sd = p.side[si];
@@ -125,141 +158,207 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const __grid_c
     const double t = p.inv_freq[i] * kInvTwoPi;
     turn_s[i] = (unsigned long long)((t - floor(t)) * 18446744073709551616.0);
   }
+  for (int d = tid; d < p.D; d += kQkThreads) w_s[d] = sd.w ? weight_at(p, sd.w, d) : 1.f;
   __syncthreads();
   const int lpr = p.lpr, sub = lane & (lpr - 1), gpw = 32 / lpr;   // groups per warp
   const int units = p.D / (2 * V), ru = p.rot / (2 * V);
   int o1[UPL], o2[UPL];
   bool has[UPL];
-  float w1[UPL][V], w2[UPL][V], dw1[UPL][V], dw2[UPL][V];
+  float dw1[UPL][V], dw2[UPL][V];
 #pragma unroll
   for (int i = 0; i < UPL; ++i) {
     const int u = sub + i * 32;
     has[i] = u < units;
     unit_at<V, INTER>(p, has[i] ? u : 0, o1[i], o2[i]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      w1[i][j] = sd.w ? weight_at(p, sd.w, o1[i] + j) : 1.f;
-      w2[i][j] = sd.w ? weight_at(p, sd.w, o2[i] + j) : 1.f;
-      dw1[i][j] = dw2[i][j] = 0.f;
-    }
+    for (int j = 0; j < V; ++j) dw1[i][j] = dw2[i][j] = 0.f;
   }
   const int64_t items = (int64_t)p.B * p.L * sd.hsplit;
   const int64_t step = (int64_t)sd.ctas * (kQkThreads / 32) * gpw;
+  const int64_t first = ((int64_t)(blockIdx.x - sd.cta0) * (kQkThreads / 32) + warp) * gpw;
   const float inv_d = 1.f / (float)p.D;
-  for (int64_t it0 = ((int64_t)(blockIdx.x - sd.cta0) * (kQkThreads / 32) + warp) * gpw; it0 < items; it0 += step) {
-    const int64_t it = it0 + lane / lpr;
-    const bool live = it < items;
-    const int64_t tok = (live ? it : 0) / sd.hsplit;
-    const int h0 = (int)((live ? it : 0) - tok * sd.hsplit) * sd.hpg, h1 = live ? min(sd.H, h0 + sd.hpg) : h0;
-    const int64_t b = tok / p.L, l = tok - b * p.L;
-    const int64_t po = b * p.pos_b + l * p.pos_l;
-    const long long pos = p.pos64 ? static_cast<const long long*>(p.pos)[po] : (long long)static_cast<const int*>(p.pos)[po];
-    float cs[UPL][V], sn[UPL][V];
+
+  // A walk over this group's rows: item after item (a token and up to hpg of its heads), the same number of steps in the
+  // whole warp.  `left` heads of the current item are real.
+  struct Walk { int64_t it0; int hh, left; const T* x; const T* g; };
+  auto decode = [&](int64_t it0, int64_t& tok, int64_t& b, int64_t& l, int& h0) {
+    int64_t it = it0 + lane / lpr;
+    if (it >= items) it = 0;
+    if (items <= 0x7fffffff) {                                    // 32-bit divisions are several times cheaper
+      const uint32_t t = (uint32_t)it / (uint32_t)sd.hsplit, bb = t / (uint32_t)p.L;
+      tok = t; b = bb; l = t - bb * (uint32_t)p.L;
+      h0 = (int)((uint32_t)it - t * (uint32_t)sd.hsplit) * sd.hpg;
+    } else {
+      tok = it / sd.hsplit; b = tok / p.L; l = tok - b * p.L;
+      h0 = (int)(it - tok * sd.hsplit) * sd.hpg;
+    }
+    return it0 + lane / lpr < items ? min(sd.H - h0, sd.hpg) : 0;
+  };
+  auto enter = [&](Walk& w) {
+    int64_t tok, b, l;
+    int h0;
+    w.left = decode(w.it0, tok, b, l, h0);
+    w.hh = sd.hpg;
+    w.x = static_cast<const T*>(sd.x) + b * sd.xb + l * sd.xl + h0 * sd.xh;
+    if (BWD) w.g = static_cast<const T*>(sd.g) + b * sd.gb + l * sd.gl + h0 * sd.gh;
+  };
+  auto advance = [&](Walk& w) {
+    --w.left;
+    w.x += sd.xh;
+    if (BWD) w.g += sd.gh;
+    if (--w.hh == 0) {
+      w.it0 += step;
+      if (w.it0 < items) enter(w);
+    }
+  };
+  auto slot = [&](int stage, int part) { return ring + ((size_t)(stage * kParts + part) * kQkThreads + tid) * kBytes; };
+  auto issue = [&](Walk& w, int stage) {
+    if (w.it0 < items) {
+      if (w.left > 0 && has[0]) {
+        if (!BWD || sd.w) {
+          copy_async<kBytes>(slot(stage, 0), w.x + o1[0]);
+          copy_async<kBytes>(slot(stage, 1), w.x + o2[0]);
+        }
+        if constexpr (BWD) {
+          copy_async<kBytes>(slot(stage, kParts - 2), w.g + o1[0]);
+          copy_async<kBytes>(slot(stage, kParts - 1), w.g + o2[0]);
+        }
+      }
+      advance(w);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  Walk ahead = {first, 0, 0, nullptr, nullptr};                   // loads; without asynchronous copies the row in hand
+  if (first < items) enter(ahead);
+  if constexpr (kAsync)
+    for (int s = 0; s < kQkStages; ++s) issue(ahead, s);
+  int64_t it0 = first;                                            // the item in hand
+  int stage = 0, hh = 0, left = 0;
+  T* y = nullptr;
+  float cs[UPL][V], sn[UPL][V];
+  while (it0 < items) {
+    if (hh == 0) {
+      int64_t tok, b, l;
+      int h0;
+      left = decode(it0, tok, b, l, h0);
+      y = static_cast<T*>(sd.out) + (tok * sd.H + h0) * (int64_t)p.D;
+      const int64_t po = b * p.pos_b + l * p.pos_l;
+      const long long pos = p.pos64 ? static_cast<const long long*>(p.pos)[po] : (long long)static_cast<const int*>(p.pos)[po];
+#pragma unroll
+      for (int i = 0; i < UPL; ++i) {
+        const int u = sub + i * 32;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          cs[i][j] = 1.f;
+          sn[i][j] = 0.f;
+          if (u < ru) {
+            const long long frac = (long long)(turn_s[u * V + j] * (unsigned long long)pos);
+            sincospif((float)frac * 1.0842021724855044e-19f, &sn[i][j], &cs[i][j]);    // 2^-63: twice the fraction of a turn
+            cs[i][j] *= p.scaling;
+            sn[i][j] *= p.scaling;
+          }
+        }
+      }
+    }
+    const bool on = hh < left;
+    float a[UPL][V], c[UPL][V], ga[BWD ? UPL : 1][V], gc[BWD ? UPL : 1][V];
+    if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(kQkStages - 1) : "memory");
 #pragma unroll
     for (int i = 0; i < UPL; ++i) {
-      const int u = sub + i * 32;
-      const bool turns = u < ru;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        cs[i][j] = 1.f;
-        sn[i][j] = 0.f;
-        if (turns) {
-          const long long frac = (long long)(turn_s[u * V + j] * (unsigned long long)pos);
-          sincospif((float)frac * 1.0842021724855044e-19f, &sn[i][j], &cs[i][j]);    // 2^-63: twice the fraction of a turn
-          cs[i][j] *= p.scaling;
-          sn[i][j] *= p.scaling;
+        a[i][j] = c[i][j] = 0.f;
+        if (BWD) ga[i][j] = gc[i][j] = 0.f;
+      }
+      if (on && has[i]) {
+        if (!BWD || sd.w) {
+          const T* x = ahead.x;
+          load_v<T, V>(kAsync ? reinterpret_cast<const T*>(slot(stage, 0)) : x + o1[i], a[i]);
+          load_v<T, V>(kAsync ? reinterpret_cast<const T*>(slot(stage, 1)) : x + o2[i], c[i]);
+        }
+        if constexpr (BWD) {
+          const T* g = ahead.g;
+          load_v<T, V>(kAsync ? reinterpret_cast<const T*>(slot(stage, kParts - 2)) : g + o1[i], ga[i]);
+          load_v<T, V>(kAsync ? reinterpret_cast<const T*>(slot(stage, kParts - 1)) : g + o2[i], gc[i]);
         }
       }
     }
-    const T* x0 = static_cast<const T*>(sd.x) + b * sd.xb + l * sd.xl;
-    const T* g0 = BWD ? static_cast<const T*>(sd.g) + b * sd.gb + l * sd.gl : nullptr;
-    T* y0 = static_cast<T*>(sd.out) + tok * sd.H * (int64_t)p.D;
-    for (int hh = 0; hh < sd.hpg; hh += kHeads) {               // the same trip count in the whole warp
-      float a[kHeads][UPL][V], c[kHeads][UPL][V], ga[BWD ? kHeads : 1][UPL][V], gc[BWD ? kHeads : 1][UPL][V];
-      float ss[kHeads], dot[kHeads];
+    float ss = 0.f, dot = 0.f, gw1[BWD ? UPL : 1][V], gw2[BWD ? UPL : 1][V];
 #pragma unroll
-      for (int k = 0; k < kHeads; ++k) {
-        const int h = h0 + hh + k;
-        const bool on = h < h1;
+    for (int i = 0; i < UPL; ++i) {
+      float w1[V], w2[V];
+      if constexpr (BWD) {
+        rotate<V, INTER, true>(ga[i], gc[i], cs[i], sn[i]);
+        load_v<float, V>(w_s + o1[i], w1);
+        load_v<float, V>(w_s + o2[i], w2);
+      }
 #pragma unroll
-        for (int i = 0; i < UPL; ++i) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            a[k][i][j] = c[k][i][j] = 0.f;
-            if (BWD) ga[k][i][j] = gc[k][i][j] = 0.f;
-          }
-          if (on && has[i]) {
-            if (!BWD || sd.w) {
-              load_v<T, V>(x0 + h * sd.xh + o1[i], a[k][i]);
-              load_v<T, V>(x0 + h * sd.xh + o2[i], c[k][i]);
-            }
-            if constexpr (BWD) {
-              load_v<T, V>(g0 + h * sd.gh + o1[i], ga[k][i]);
-              load_v<T, V>(g0 + h * sd.gh + o2[i], gc[k][i]);
-            }
-          }
+      for (int j = 0; j < V; ++j) {
+        ss = fmaf(a[i][j], a[i][j], fmaf(c[i][j], c[i][j], ss));
+        if constexpr (BWD) {
+          gw1[i][j] = ga[i][j] * w1[j];
+          gw2[i][j] = gc[i][j] * w2[j];
+          dot = fmaf(gw1[i][j], a[i][j], fmaf(gw2[i][j], c[i][j], dot));
         }
       }
-#pragma unroll
-      for (int k = 0; k < kHeads; ++k) {
-        ss[k] = dot[k] = 0.f;
-#pragma unroll
-        for (int i = 0; i < UPL; ++i) {
-          if constexpr (BWD) rotate<V, INTER, true>(ga[k][i], gc[k][i], cs[i], sn[i]);
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            ss[k] = fmaf(a[k][i][j], a[k][i][j], fmaf(c[k][i][j], c[k][i][j], ss[k]));
-            if constexpr (BWD) dot[k] = fmaf(ga[k][i][j] * w1[i][j], a[k][i][j], fmaf(gc[k][i][j] * w2[i][j], c[k][i][j], dot[k]));
-          }
-        }
+    }
+    if (sd.w) {
+      for (int o = lpr >> 1; o > 0; o >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (BWD) dot += __shfl_xor_sync(0xffffffffu, dot, o);
       }
-      if (sd.w) {
-        for (int o = lpr >> 1; o > 0; o >>= 1)
+    }
+    if constexpr (kAsync) {
+      issue(ahead, stage);                                        // the slot's values are in registers now
+      if (++stage == kQkStages) stage = 0;
+    }
+    const float rstd = sd.w ? rsqrtf(fmaf(ss, inv_d, p.eps)) : 1.f;
+    const float m = BWD ? dot * inv_d * rstd * rstd : 0.f;
 #pragma unroll
-          for (int k = 0; k < kHeads; ++k) {
-            ss[k] += __shfl_xor_sync(0xffffffffu, ss[k], o);
-            if (BWD) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
-          }
+    for (int i = 0; i < UPL; ++i) {
+      float y1[V], y2[V], w1[V], w2[V];
+      if constexpr (!BWD) {
+        load_v<float, V>(w_s + o1[i], w1);
+        load_v<float, V>(w_s + o2[i], w2);
       }
 #pragma unroll
-      for (int k = 0; k < kHeads; ++k) {
-        const int h = h0 + hh + k;
-        const bool on = h < h1;
-        const float rstd = sd.w ? rsqrtf(fmaf(ss[k], inv_d, p.eps)) : 1.f;
-        const float m = BWD ? dot[k] * inv_d * rstd * rstd : 0.f;
-#pragma unroll
-        for (int i = 0; i < UPL; ++i) {
-          float y1[V], y2[V];
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            if constexpr (BWD) {
-              y1[j] = ga[k][i][j];
-              y2[j] = gc[k][i][j];
-              if (sd.w) {
-                if (on) {                                       // rows past the end hold zeros, and rstd of a zero row is large
-                  dw1[i][j] = fmaf(ga[k][i][j], a[k][i][j] * rstd, dw1[i][j]);
-                  dw2[i][j] = fmaf(gc[k][i][j], c[k][i][j] * rstd, dw2[i][j]);
-                }
-                y1[j] = rstd * (ga[k][i][j] * w1[i][j] - a[k][i][j] * m);
-                y2[j] = rstd * (gc[k][i][j] * w2[i][j] - c[k][i][j] * m);
-              }
-            } else {
-              y1[j] = a[k][i][j] * rstd * w1[i][j];
-              y2[j] = c[k][i][j] * rstd * w2[i][j];
+      for (int j = 0; j < V; ++j) {
+        if constexpr (BWD) {
+          y1[j] = ga[i][j];
+          y2[j] = gc[i][j];
+          if (sd.w) {
+            if (on) {                                             // rows past the end hold zeros, and rstd of a zero row is large
+              dw1[i][j] = fmaf(ga[i][j], a[i][j] * rstd, dw1[i][j]);
+              dw2[i][j] = fmaf(gc[i][j], c[i][j] * rstd, dw2[i][j]);
             }
+            y1[j] = rstd * (gw1[i][j] - a[i][j] * m);
+            y2[j] = rstd * (gw2[i][j] - c[i][j] * m);
           }
-          if constexpr (!BWD) rotate<V, INTER, false>(y1, y2, cs[i], sn[i]);
-          if (on && has[i]) {
-            store_v<T, V>(y0 + h * (int64_t)p.D + o1[i], y1);
-            store_v<T, V>(y0 + h * (int64_t)p.D + o2[i], y2);
-          }
+        } else {
+          y1[j] = a[i][j] * rstd * w1[j];
+          y2[j] = c[i][j] * rstd * w2[j];
         }
       }
+      if constexpr (!BWD) rotate<V, INTER, false>(y1, y2, cs[i], sn[i]);
+      if (on && has[i]) {
+        store_v<T, V>(y + o1[i], y1);
+        store_v<T, V>(y + o2[i], y2);
+      }
+    }
+    if constexpr (!kAsync) advance(ahead);
+    y += p.D;
+    if (++hh == sd.hpg) {
+      hh = 0;
+      it0 += step;
     }
   }
+  if constexpr (kAsync) asm volatile("cp.async.wait_group 0;" ::: "memory");
   if constexpr (BWD) {
     if (sd.w) {
       // the CTA's share of dw, summed in a fixed order: over the groups of a warp, then over the warps
+      float* dw_s = reinterpret_cast<float*>(ring);               // the copies are done: their slots are free
+      __syncthreads();
 #pragma unroll
       for (int i = 0; i < UPL; ++i)
 #pragma unroll
@@ -269,14 +368,14 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const __grid_c
             dw2[i][j] += __shfl_xor_sync(0xffffffffu, dw2[i][j], o);
           }
           if (lane < lpr && has[i]) {
-            dw_s[warp][o1[i] + j] = dw1[i][j];
-            dw_s[warp][o2[i] + j] = dw2[i][j];
+            dw_s[warp * kQkMaxD + o1[i] + j] = dw1[i][j];
+            dw_s[warp * kQkMaxD + o2[i] + j] = dw2[i][j];
           }
         }
       __syncthreads();
       for (int d = tid; d < p.D; d += kQkThreads) {
         float s = 0.f;
-        for (int w = 0; w < kQkThreads / 32; ++w) s += dw_s[w][d];
+        for (int w = 0; w < kQkThreads / 32; ++w) s += dw_s[w * kQkMaxD + d];
         sd.dw[(int64_t)(blockIdx.x - sd.cta0) * p.D + d] = s;
       }
     }
@@ -305,12 +404,15 @@ __global__ void __launch_bounds__(256) qk_weight_grad_kernel(QkSumParams p) {
   }
 }
 
-// CTAs of one side: enough to fill the device, never more than there are rows for
-constexpr int kQkMaxCtas = 148 * 8;
+// CTAs of a call: one wave at two per SM (more of them cost 2 to 19 % at 64K tokens), never more than there are rows for
+constexpr int kQkMaxCtas = 148 * 2;
 
 template <typename T, int V, int UPL, bool INTER, bool BWD>
 static void launch_qk(const QkParams& p, int ctas, cudaStream_t st) {
-  qk_norm_rope_kernel<T, V, UPL, INTER, BWD><<<ctas, kQkThreads, 0, st>>>(p);
+  constexpr size_t smem = qk_smem<T, V, UPL, BWD>();
+  if (smem > 48 * 1024)
+    cudaFuncSetAttribute(qk_norm_rope_kernel<T, V, UPL, INTER, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  qk_norm_rope_kernel<T, V, UPL, INTER, BWD><<<ctas, kQkThreads, smem, st>>>(p);
 }
 
 template <typename T, bool INTER, bool BWD>

@@ -534,16 +534,17 @@ def _host_ids(x, what: str) -> torch.Tensor:
 
 def _pool_layers(k_pages, v_pages, what: str):
     """(layers, pages per layer, bytes from layer to layer) of two pools (num_layers, num_pages, h_kv, S, D) or one layer of them."""
-    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.stride() != v_pages.stride():
+    shape, stride = k_pages.shape, k_pages.stride()
+    if shape != v_pages.shape or k_pages.dtype != v_pages.dtype or stride != v_pages.stride():
         raise ValueError(f"{what}: k_pages and v_pages differ in shape, type or strides")
-    if k_pages.dim() not in (4, 5):
-        raise ValueError(f"{what}: pools are (num_pages, h_kv, S, D) or (num_layers, num_pages, h_kv, S, D), got {tuple(k_pages.shape)}")
-    layers = k_pages.shape[0] if k_pages.dim() == 5 else 1
-    first = k_pages[0] if k_pages.dim() == 5 else k_pages
-    if not first.is_contiguous():
+    if len(shape) not in (4, 5):
+        raise ValueError(f"{what}: pools are (num_pages, h_kv, S, D) or (num_layers, num_pages, h_kv, S, D), got {tuple(shape)}")
+    pages, h, S, D = shape[-4:]
+    if pages * h * S * D and stride[-4:] != (h * S * D, S * D, D, 1):
         raise ValueError(f"{what}: a layer's pool must be contiguous")
-    step = k_pages.stride(0) if k_pages.dim() == 5 else first.numel()
-    return layers, first.shape[0], step * k_pages.element_size()
+    if len(shape) == 4:
+        return 1, pages, pages * h * S * D * k_pages.element_size()
+    return shape[0], pages, stride[0] * k_pages.element_size()
 
 
 def copy_pages(k_pages, v_pages, src, dst) -> None:
@@ -712,34 +713,39 @@ def _rope_rows(x):
 def _rope_call(name, sides, pos, inv_freq, interleaved, scaling, eps, w_dtype, ws=None):
     """sides: (x or None, weight, out, d_out, d_weight) of each tensor."""
     B, L, _, D = sides[0][2].shape
-    t = (_lib.RopeTensor * len(sides))()
-    for r, (x, w, out, g, dw) in zip(t, sides):
-        r.x, r.weight, r.out, r.d_out, r.d_weight = ptr(x), ptr(w), ptr(out), ptr(g), ptr(dw)
-        if x is not None:
-            r.x_stride_b, r.x_stride_l, r.x_stride_h = x.stride()[:3]
-        if g is not None:
-            r.g_stride_b, r.g_stride_l, r.g_stride_h = g.stride()[:3]
-        r.heads = out.shape[2]
-    ps = pos.stride() if pos.dim() == 2 else (0, pos.stride(0))
-    args = [t, len(sides), ptr(pos) if pos.numel() else None, int(pos.dtype == torch.int64), 0 if pos.dim() == 2 and pos.shape[0] == 1 else ps[0],
-            ps[1], ptr(inv_freq), 2 * inv_freq.numel(), B, L, D, int(interleaved), scaling, eps, dtype_code(sides[0][2]), w_dtype]
+    none = (0, 0, 0)
+    t = (_lib.RopeTensor * len(sides))(*[
+        (ptr(x), ptr(w), ptr(out), ptr(g), ptr(dw), *(none if x is None else x.stride()[:3]), *(none if g is None else g.stride()[:3]),
+         out.shape[2], 0) for x, w, out, g, dw in sides])
+    pb, pl = (0, pos.stride(0)) if pos.dim() == 1 else pos.stride()
+    if pos.dim() == 2 and pos.shape[0] == 1:
+        pb = 0
+    args = (t, len(sides), ptr(pos) if pos.numel() else None, pos.dtype == torch.int64, pb, pl, ptr(inv_freq), 2 * inv_freq.shape[0], B, L, D,
+            interleaved, scaling, eps, dtype_code(sides[0][2]), w_dtype)
     if ws is not None:
-        args += [ptr(ws), ws.numel()]
+        args += (ptr(ws), ws.numel())
     call(name, *args, stream())
+
+
+def _rope_forward(q, k, q_weight, k_weight, positions, inv_freq, interleaved, scaling, eps):
+    """(inputs as read, weights, outputs, type of the weights) of the tensors given."""
+    xs = [_rope_rows(q)] if k is None else [_rope_rows(q), _rope_rows(k)]
+    ws = (q_weight, k_weight)
+    outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+    w = q_weight if q_weight is not None else (k_weight if k is not None else None)
+    w_dtype = F32 if w is None else dtype_code(w)
+    _rope_call("hils_qk_norm_rope_fwd", [(x, w, o, None, None) for x, w, o in zip(xs, ws, outs)], positions, inv_freq, interleaved, scaling, eps,
+               w_dtype)
+    return xs, ws, outs, w_dtype
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, interleaved, scaling, eps):
-        xs = [_rope_rows(x) for x in (q, k) if x is not None]
-        ws = [w for x, w in ((q, q_weight), (k, k_weight)) if x is not None]
-        outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
-        w_dtype = next((dtype_code(w) for w in ws if w is not None), F32)
-        _rope_call("hils_qk_norm_rope_fwd", [(x, w, o, None, None) for x, w, o in zip(xs, ws, outs)], positions, inv_freq, interleaved, scaling,
-                   eps, w_dtype)
+        xs, ws, outs, w_dtype = _rope_forward(q, k, q_weight, k_weight, positions, inv_freq, interleaved, scaling, eps)
         # without a norm the backward is the rotation back, which does not read x
         ctx.save_for_backward(positions, inv_freq, *[t for x, w in zip(xs, ws) if w is not None for t in (x, w)])
-        ctx.meta = ([w is not None for w in ws], [(x.shape, x.dtype) for x in xs], interleaved, scaling, eps, w_dtype)
+        ctx.meta = ([w is not None for _, w in zip(xs, ws)], [(x.shape, x.dtype) for x in xs], interleaved, scaling, eps, w_dtype)
         return outs[0], (outs[1] if k is not None else None)
 
     @staticmethod
@@ -796,7 +802,11 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: f
         inv_freq = inv_freq.double().contiguous()
     if positions.data_ptr() % 16:
         positions = positions.clone()
-    return _QkNormRope.apply(q, k, q_weight, k_weight, positions, inv_freq, bool(interleaved), float(attention_scaling), float(eps))
+    args = (q, k, q_weight, k_weight, positions, inv_freq, bool(interleaved), float(attention_scaling), float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        return _QkNormRope.apply(*args)
+    outs = _rope_forward(*args)[2]
+    return outs[0], (outs[1] if k is not None else None)
 
 
 class _ExactChunkLogZ(torch.autograd.Function):
