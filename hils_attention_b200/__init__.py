@@ -8,12 +8,12 @@ attention module does; `cache` is the KV store used for prefill and decode, `kv_
 from . import _lib
 from .naive_bsa import naive_bsa_kernel
 from .ops import (HiLS_block_M_head, chunk_attn_pool, chunk_attn_pool_tilelang, chunk_mean_pool,
-                  commit_drafts, copy_pages, exact_chunk_log_z_tl, flex_attn_tl, flex_attn_tl_two_phase, inter_chunk_softmax,
+                  commit_drafts, copy_pages, draft_positions, exact_chunk_log_z_tl, flex_attn_tl, flex_attn_tl_two_phase, inter_chunk_softmax,
                   online_softmax_topk_head, qk_norm_rope, rmsnorm_rope, rope_frequencies, rope_rotary_pos_emb, single_tensor_rope_autograd,
-                  sparse_attn_combine)
+                  sparse_attn_combine, tree_attn_paged)
 
 __all__ = ["HiLS_block_M_head", "chunk_attn_pool", "chunk_attn_pool_tilelang", "chunk_mean_pool",
-           "commit_drafts", "copy_pages",
+           "commit_drafts", "copy_pages", "draft_positions",
            "exact_chunk_log_z_tl", "flex_attn_tl", "flex_attn_tl_two_phase", "inter_chunk_softmax",
            "online_softmax_topk_head", "qk_norm_rope", "rmsnorm_rope", "rope_frequencies", "rope_rotary_pos_emb", "single_tensor_rope_autograd",
-           "sparse_attn_combine", "naive_bsa_kernel"]
+           "sparse_attn_combine", "tree_attn_paged", "naive_bsa_kernel"]

@@ -1,6 +1,8 @@
 // Error text of the C ABI (one buffer per host thread) and library identification.
 #include <stdarg.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 
 namespace hils {
@@ -29,6 +31,7 @@ int take_status_topk_tc();
 int take_status_logz_tc();
 int take_status_paged();
 int take_status_pages();
+int take_status_tree();
 }  // namespace hils
 
 extern "C" int hils_version(void) { return 100; }
@@ -43,7 +46,11 @@ extern "C" int hils_take_device_status(void) {
   const int e = hils::take_status_logz_tc();
   const int f = hils::take_status_paged();
   const int g = hils::take_status_pages();
-  if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0 || f < 0 || g < 0) return -1;
-  return a != 0 ? a : (b != 0 ? b : (c != 0 ? c : (d != 0 ? d : (e != 0 ? e : (f != 0 ? f : g)))));
+  const int h = hils::take_status_tree();
+  for (const int v : {a, b, c, d, e, f, g, h})
+    if (v < 0) return -1;
+  for (const int v : {a, b, c, d, e, f, g, h})
+    if (v != 0) return v;
+  return 0;
 }
 extern "C" const char* hils_last_error(void) { return hils::g_err; }

@@ -1,0 +1,337 @@
+// Attention of a tree of drafted tokens over the paged store (tree_common.cuh states what a row sees).
+//
+// CUDA-core kernel: one CTA per (sequence, key head, 32 rows, share of the tiles).  K and V tiles of 64 keys are brought to
+// shared memory as fp32; a thread forms 2 x 4 scores and 2 x D/16 outputs from registers; running maximum and sum per row.
+#include <algorithm>
+
+#include "tree_common.cuh"
+
+namespace hils {
+
+// Set when a page table holds an id outside the pool or a sequence reaches past the table's width; the tile is skipped.
+static __device__ int g_tree_status = 0;
+
+constexpr int kTreeThreads = 256, kTreeRows = 32;
+
+template <int D>
+constexpr size_t tree_smem_floats() { return (size_t)kTreeRows * D + 64 * (D + 4) + 64 * D + kTreeRows * 65 + kTreeRows; }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeParams p) {
+  constexpr int CPT = D / 16;                             // output columns of a thread: float4 at 4 tx, and 64 + 4 tx
+  __shared__ int par_s[2][kTreeMaxNodes];
+  __shared__ u64t anc_s[2][kTreeMaxNodes], vis_s[kTreeRows];
+  __shared__ int lo_s[kTreeRows];
+  __shared__ u64t dmask_s[kTreeRows];
+  extern __shared__ __align__(16) float tsm[];
+  float* q_s = tsm;                                       // [32][D]
+  float* k_s = q_s + kTreeRows * D;                       // [64][D + 4]
+  float* v_s = k_s + 64 * (D + 4);                        // [64][D]
+  float* s_s = v_s + 64 * D;                              // [32][65]
+  float* corr_s = s_s + kTreeRows * 65;                   // [32]
+  const int tid = threadIdx.x, G = p.h_q / p.h_kv, R = p.n * G;
+  const int rb = blockIdx.x % p.row_blocks, split = blockIdx.x / p.row_blocks, h = blockIdx.y, b = blockIdx.z;
+  bool over;
+  const int len = tree_length(p, b, over);
+  if (over && tid == 0) atomicExch(&g_tree_status, 8200002);
+  tree_ancestors(p.parents + (int64_t)b * p.n, p.n, par_s, anc_s, tid);
+  const u64t* anc = anc_s[0];
+  if (tid < kTreeRows) {
+    const int row = rb * kTreeRows + tid, j = row / G;
+    const bool there = row < R && anc[j] != 0ull;
+    const int lo = there ? tree_low(p, len + __popcll(anc[j]) - 1) : 0x7fffffff;
+    lo_s[tid] = lo;
+    dmask_s[tid] = there ? tree_draft_mask(p, anc, j, len, lo) : 0ull;
+  }
+  const int64_t new0 = (int64_t)b * p.n;
+  for (int x = tid; x < kTreeRows * (D / 4); x += kTreeThreads) {
+    const int r = x / (D / 4), d = (x - r * (D / 4)) * 4, row = rb * kTreeRows + r;
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < R) f = load4(static_cast<const T*>(p.q) + ((new0 + row / G) * p.h_q + h * G + row % G) * D + d);
+    *reinterpret_cast<float4*>(q_s + r * D + d) = f;
+  }
+  const int c0 = tree_low(p, len) >> 6, c1 = (len + 63) >> 6;
+  const int nt = 1 + max(0, c1 - c0), per = (nt + p.splits - 1) / p.splits;
+  const int t0 = split * per, t1 = min(nt, t0 + per);
+  const int ty = tid >> 4, tx = tid & 15, sr = tid >> 3, sl = tid & 7;
+  float acc[2][CPT], m_run = -CUDART_INF_F, l_run = 0.f;   // m_run, l_run: of row sr, the same in its eight threads
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int e = 0; e < CPT; ++e) acc[i][e] = 0.f;
+  for (int t = t0; t < t1; ++t) {
+    const int c = c0 + t - 1;
+    const int pg = t > 0 ? tree_page(p, b, c) : 0;
+    if (pg < 0) {
+      if (tid == 0) atomicExch(&g_tree_status, 8200001);
+      continue;
+    }
+    __syncthreads();
+    if (tid < kTreeRows) vis_s[tid] = t == 0 ? dmask_s[tid] : tree_page_mask(p, c, len, lo_s[tid]);
+    // keys nobody may see hold anything, NaN too: their V rows become zeros
+    const u64t held = t == 0 ? (p.n >= 64 ? ~0ull : (1ull << p.n) - 1) : tree_page_mask(p, c, len, 0);
+    const T* kb = t == 0 ? static_cast<const T*>(p.k_new) + (new0 * p.h_kv + h) * D : static_cast<const T*>(p.k_pages) + ((int64_t)pg * p.h_kv + h) * 64 * D;
+    const T* vb = t == 0 ? static_cast<const T*>(p.v_new) + (new0 * p.h_kv + h) * D : static_cast<const T*>(p.v_pages) + ((int64_t)pg * p.h_kv + h) * 64 * D;
+    const int64_t rs = t == 0 ? (int64_t)p.h_kv * D : D;
+    for (int x = tid; x < 64 * (D / 4); x += kTreeThreads) {
+      const int r = x / (D / 4), d = (x - r * (D / 4)) * 4;
+      float4 kf = make_float4(0.f, 0.f, 0.f, 0.f), vf = kf;
+      if (held >> r & 1ull) {
+        kf = load4(kb + r * rs + d);
+        vf = load4(vb + r * rs + d);
+      }
+      *reinterpret_cast<float4*>(k_s + r * (D + 4) + d) = kf;
+      *reinterpret_cast<float4*>(v_s + r * D + d) = vf;
+    }
+    __syncthreads();
+    // scores of rows 2 ty, 2 ty + 1 against keys tx, tx + 16, tx + 32, tx + 48
+    float s[2][4] = {};
+    for (int d = 0; d < D; d += 4) {
+      const float4 qa = *reinterpret_cast<const float4*>(q_s + (2 * ty) * D + d), qb = *reinterpret_cast<const float4*>(q_s + (2 * ty + 1) * D + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 kf = *reinterpret_cast<const float4*>(k_s + (tx + 16 * i) * (D + 4) + d);
+        s[0][i] = fmaf(qa.x, kf.x, fmaf(qa.y, kf.y, fmaf(qa.z, kf.z, fmaf(qa.w, kf.w, s[0][i]))));
+        s[1][i] = fmaf(qb.x, kf.x, fmaf(qb.y, kf.y, fmaf(qb.z, kf.z, fmaf(qb.w, kf.w, s[1][i]))));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s_s[(2 * ty) * 65 + tx + 16 * i] = s[0][i];
+      s_s[(2 * ty + 1) * 65 + tx + 16 * i] = s[1][i];
+    }
+    __syncthreads();
+    {
+      const u64t vis = vis_s[sr];
+      float y[8], top = -CUDART_INF_F;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = sl + 8 * i;
+        y[i] = (vis >> key & 1ull) ? s_s[sr * 65 + key] * p.scale : -CUDART_INF_F;
+        top = fmaxf(top, y[i]);
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float mn = fmaxf(m_run, top), ref = mn > -CUDART_INF_F ? mn : 0.f;     // a row whose scores are NaN stays NaN
+      const float corr = m_run > -CUDART_INF_F ? expf(m_run - ref) : 0.f;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = sl + 8 * i;
+        const float e = (vis >> key & 1ull) ? expf(y[i] - ref) : 0.f;
+        s_s[sr * 65 + key] = e;
+        sum += e;
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      l_run = l_run * corr + sum;
+      m_run = mn;
+      if (sl == 0) corr_s[sr] = corr;
+    }
+    __syncthreads();
+    const float ca = corr_s[2 * ty], cb = corr_s[2 * ty + 1];
+#pragma unroll
+    for (int e = 0; e < CPT; ++e) { acc[0][e] *= ca; acc[1][e] *= cb; }
+    const u64t va = vis_s[2 * ty], vbits = vis_s[2 * ty + 1];
+    const bool mixed = va != held || vbits != held;       // a key that one row sees and another does not may hold NaN
+    for (int key = 0; key < 64; ++key) {
+      const float pa = s_s[(2 * ty) * 65 + key], pb = s_s[(2 * ty + 1) * 65 + key];
+      float v[CPT];
+#pragma unroll
+      for (int e = 0; e < CPT; e += 4) *reinterpret_cast<float4*>(v + e) = *reinterpret_cast<const float4*>(v_s + key * D + e * 16 + tx * 4);
+      if (!mixed) {
+#pragma unroll
+        for (int e = 0; e < CPT; ++e) { acc[0][e] = fmaf(pa, v[e], acc[0][e]); acc[1][e] = fmaf(pb, v[e], acc[1][e]); }
+      } else {
+        if (va >> key & 1ull)
+#pragma unroll
+          for (int e = 0; e < CPT; ++e) acc[0][e] = fmaf(pa, v[e], acc[0][e]);
+        if (vbits >> key & 1ull)
+#pragma unroll
+          for (int e = 0; e < CPT; ++e) acc[1][e] = fmaf(pb, v[e], acc[1][e]);
+      }
+    }
+  }
+  __syncthreads();
+  float* ml_s = s_s;                                      // [32][2]: max and sum of a row
+  if (sl == 0) { ml_s[2 * sr] = m_run; ml_s[2 * sr + 1] = l_run; }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 2 * ty + i, row = rb * kTreeRows + r;
+    if (row >= R) continue;
+    const float m = ml_s[2 * r], l = ml_s[2 * r + 1];
+    const int64_t out = (new0 + row / G) * p.h_q + h * G + row % G;
+    if (p.splits == 1) {
+      const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+#pragma unroll
+      for (int e = 0; e < CPT; e += 4)
+        store4(static_cast<T*>(p.o) + out * D + e * 16 + tx * 4,
+               make_float4(acc[i][e] * inv, acc[i][e + 1] * inv, acc[i][e + 2] * inv, acc[i][e + 3] * inv));
+      if (tx == 0) p.lse[out] = l > 0.f ? m + logf(l) : (l == l ? -CUDART_INF_F : l);
+    } else {
+      const int64_t at = (int64_t)split * p.B * p.n * p.h_q + out;
+#pragma unroll
+      for (int e = 0; e < CPT; e += 4)
+        store4(p.part_o + at * D + e * 16 + tx * 4, make_float4(acc[i][e], acc[i][e + 1], acc[i][e + 2], acc[i][e + 3]));
+      if (tx == 0) { p.part_ml[2 * at] = m * kLog2E; p.part_ml[2 * at + 1] = l; }
+    }
+  }
+}
+
+// Joins the splits: o = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  One warp per row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = (int64_t)p.B * p.n * p.h_q, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  float top = -CUDART_INF_F;
+  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_ml[2 * (s * rows + row)]);
+  top = warp_max(top);
+  const float ref = top > -CUDART_INF_F ? top : 0.f;
+  float acc[D / 32], l = 0.f;
+#pragma unroll
+  for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const int64_t at = s * rows + row;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+    if (ml.y == 0.f) continue;                            // nothing visible in this share
+    const float w = exp2f(ml.x - ref);
+    l = fmaf(w, ml.y, l);
+#pragma unroll
+    for (int e = 0; e < D / 32; e += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(p.part_o + at * D + e * 32 + lane * 2);
+      acc[e] = fmaf(w, x.x, acc[e]);
+      acc[e + 1] = fmaf(w, x.y, acc[e + 1]);
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+  T* o = static_cast<T*>(p.o) + row * D;
+#pragma unroll
+  for (int e = 0; e < D / 32; e += 2) {
+    o[e * 32 + lane * 2] = from_f<T>(acc[e] * inv);
+    o[e * 32 + lane * 2 + 1] = from_f<T>(acc[e + 1] * inv);
+  }
+  if (lane == 0) p.lse[row] = l > 0.f ? (ref + log2f(l)) * kLn2F : (l == l ? -CUDART_INF_F : l);
+}
+
+// Positions of the nodes, -1 for those that are absent.
+__global__ void __launch_bounds__(kTreeMaxNodes) tree_positions_kernel(const int32_t* parents, const int32_t* lens, int32_t* pos, int n) {
+  __shared__ int par_s[2][kTreeMaxNodes];
+  __shared__ u64t anc_s[2][kTreeMaxNodes];
+  const int b = blockIdx.x, j = threadIdx.x;
+  tree_ancestors(parents + (int64_t)b * n, n, par_s, anc_s, j);
+  if (j < n) pos[(int64_t)b * n + j] = anc_s[0][j] ? max(lens[b], 0) + __popcll(anc_s[0][j]) - 1 : -1;
+}
+
+// Tiles of a sequence of at most max_len tokens
+static int tree_tiles(int max_len, int W) {
+  const int all = (max_len + 63) / 64;
+  return 1 + (W == 0 ? all : std::min<int64_t>(all, ((int64_t)W + 62) / 64 + 1));
+}
+
+// Shares of the tiles: the number that makes the busiest SM finish first, where a CTA costs what its tiles cost and about
+// four more to start and to write its partial result.
+static int tree_splits(int64_t ctas, int tiles, int slots) {
+  int best = 1;
+  int64_t cost = INT64_MAX;
+  for (int s = 1; s <= std::min(tiles, 64); ++s) {
+    const int64_t waves = (ctas * s + slots - 1) / slots, c = waves * ((tiles + s - 1) / s + 4) + (s > 1 ? 4 : 0);
+    if (c < cost) { cost = c; best = s; }
+  }
+  return best;
+}
+
+static TreeParams tree_plan(int B, int n, int h_q, int h_kv, int max_len, int W) {
+  TreeParams p = {};
+  p.B = B; p.n = n; p.h_q = h_q; p.h_kv = h_kv; p.W = W;
+  p.row_blocks = (int)(((int64_t)n * (h_q / h_kv) + kTreeRows - 1) / kTreeRows);
+  p.splits = tree_splits((int64_t)B * h_kv * p.row_blocks, tree_tiles(max_len, W), 148 * 2);
+  return p;
+}
+
+static size_t tree_workspace(const TreeParams& p, int D) {
+  return p.splits > 1 ? (size_t)p.splits * p.B * p.n * p.h_q * (D + 2) * sizeof(float) : 0;
+}
+
+int take_status_tree() {
+  int v = 0, zero = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return -1;
+  if (cudaMemcpyFromSymbol(&v, g_tree_status, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) cudaMemcpyToSymbol(g_tree_status, &zero, sizeof(int));
+  return v;
+}
+
+template <typename T, int D>
+static int launch_tree(const TreeParams& p, cudaStream_t st) {
+  const size_t smem = tree_smem_floats<D>() * sizeof(float);
+  cudaFuncSetAttribute(tree_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  tree_attn_kernel<T, D><<<dim3((unsigned)(p.row_blocks * p.splits), (unsigned)p.h_kv, (unsigned)p.B), kTreeThreads, smem, st>>>(p);
+  HILS_LAUNCH_CHECK("tree_attn_paged");
+  if (p.splits > 1) {
+    const int64_t rows = (int64_t)p.B * p.n * p.h_q;
+    tree_join_kernel<T, D><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
+    HILS_LAUNCH_CHECK("tree_attn_paged (join)");
+  }
+  return HILS_OK;
+}
+
+}  // namespace hils
+
+using namespace hils;
+
+static int check_tree(int B, int n, int h_q, int h_kv, int D, int max_len, int window_size, int chunk_size, int dtype) {
+  HILS_REQUIRE(dtype == HILS_BF16 || dtype == HILS_F32, "tree_attn_paged: dtype must be bf16 or fp32");
+  HILS_REQUIRE(B >= 0 && B <= 65535, "tree_attn_paged: %d sequences (at most 65535)", B);
+  HILS_REQUIRE(n >= 0 && n <= kTreeMaxNodes, "tree_attn_paged: %d nodes (at most %d)", n, kTreeMaxNodes);
+  HILS_REQUIRE(h_q > 0 && h_kv > 0 && h_q % h_kv == 0, "tree_attn_paged: h_q must be a multiple of h_kv");
+  HILS_REQUIRE(h_kv <= 65535 && h_q / h_kv <= 1024, "tree_attn_paged: too many heads");
+  HILS_REQUIRE(D == 64 || D == 128, "tree_attn_paged: head dimension %d (64 or 128)", D);
+  HILS_REQUIRE(chunk_size == 64, "tree_attn_paged: the page is the chunk and must hold 64 tokens (got %d)", chunk_size);
+  HILS_REQUIRE(max_len >= 0 && max_len <= 0x7fffffff - 256, "tree_attn_paged: bad length %d", max_len);
+  HILS_REQUIRE(window_size >= 0, "tree_attn_paged: negative window");
+  return HILS_OK;
+}
+
+extern "C" size_t hils_tree_attn_paged_workspace_bytes(int B, int n, int h_q, int h_kv, int D, int max_len, int window_size, int dtype) {
+  if (check_tree(B, n, h_q, h_kv, D, max_len, window_size, 64, dtype) || B == 0 || n == 0) return 0;
+  return tree_workspace(tree_plan(B, n, h_q, h_kv, max_len, window_size), D);
+}
+
+extern "C" int hils_tree_attn_paged(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages,
+                                    const int32_t* page_table, int page_stride, int num_pages, const int32_t* lens, int max_len,
+                                    const int32_t* parents, void* o, float* lse, int B, int n, int h_q, int h_kv, int D, int window_size,
+                                    int chunk_size, int mask_lmk, int expand_to_chunk, float sm_scale, int dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  if (int rc = check_tree(B, n, h_q, h_kv, D, max_len, window_size, chunk_size, dtype)) return rc;
+  HILS_REQUIRE(sm_scale > 0.f && sm_scale <= 3.4e38f, "tree_attn_paged: sm_scale must be positive");
+  HILS_REQUIRE(page_stride > 0 && num_pages > 0, "tree_attn_paged: bad size");
+  HILS_REQUIRE((max_len + 63) / 64 <= page_stride, "tree_attn_paged: %d tokens do not fit a page table of %d pages", max_len, page_stride);
+  if (B == 0 || n == 0) return HILS_OK;
+  HILS_REQUIRE(q && k_new && v_new && k_pages && v_pages && page_table && lens && parents && o && lse, "tree_attn_paged: null pointer");
+  HILS_REQUIRE(((((uintptr_t)q) | ((uintptr_t)k_new) | ((uintptr_t)v_new) | ((uintptr_t)k_pages) | ((uintptr_t)v_pages) | ((uintptr_t)o)) & 15) == 0,
+               "tree_attn_paged: tensors must be 16-byte aligned");
+  TreeParams p = tree_plan(B, n, h_q, h_kv, max_len, window_size);
+  const size_t need = tree_workspace(p, D);
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
+    set_error("tree_attn_paged: a 16-byte aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    return HILS_ERR_WORKSPACE;
+  }
+  p.q = q; p.k_new = k_new; p.v_new = v_new; p.k_pages = k_pages; p.v_pages = v_pages; p.pages = page_table; p.lens = lens;
+  p.parents = parents; p.o = o; p.lse = lse; p.page_stride = page_stride; p.num_pages = num_pages;
+  p.mask_lmk = mask_lmk; p.expand = expand_to_chunk; p.scale = sm_scale;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + (size_t)p.splits * B * n * h_q * D;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == HILS_BF16) return D == 128 ? launch_tree<bf16, 128>(p, st) : launch_tree<bf16, 64>(p, st);
+  return D == 128 ? launch_tree<float, 128>(p, st) : launch_tree<float, 64>(p, st);
+}
+
+extern "C" int hils_draft_positions(const int32_t* parents, const int32_t* lens, int32_t* positions, int B, int n, void* stream) {
+  HILS_REQUIRE(B >= 0 && n >= 0 && n <= kTreeMaxNodes, "draft_positions: %d sequences of %d nodes (at most %d)", B, n, kTreeMaxNodes);
+  if (B == 0 || n == 0) return HILS_OK;
+  HILS_REQUIRE(parents && lens && positions, "draft_positions: null pointer");
+  tree_positions_kernel<<<(unsigned)B, kTreeMaxNodes, 0, (cudaStream_t)stream>>>(parents, lens, positions, n);
+  HILS_LAUNCH_CHECK("draft_positions");
+  return HILS_OK;
+}

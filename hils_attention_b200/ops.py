@@ -510,6 +510,65 @@ def decode_step_paged(q, lmk_q, k_new, v_new, k_pages, v_pages, page_table, lens
     return (o, idx, workspace) if return_indices else (o, workspace)
 
 
+def draft_positions(parents, lens):
+    """Positions (B, n) int32 of the nodes of drafted trees: lens[b] + depth, -1 for an absent node.  parents (B, n <= 64) and
+    lens (B) int32 as in `tree_attn_paged`."""
+    if parents.dim() != 2 or parents.dtype != torch.int32 or lens.dtype != torch.int32 or lens.shape != parents.shape[:1]:
+        raise ValueError(f"draft_positions: parents (B, n) and lens (B) int32, got {tuple(parents.shape)} {parents.dtype}, "
+                         f"{tuple(lens.shape)} {lens.dtype}")
+    parents, lens = parents.contiguous(), lens.contiguous()
+    out = torch.empty_like(parents)
+    call("hils_draft_positions", ptr(parents), ptr(lens), ptr(out), parents.shape[0], parents.shape[1], stream())
+    return out
+
+
+def tree_attn_paged(q, k_new, v_new, k_pages, v_pages, page_table, lens, max_len: int, parents, window_size: Optional[int] = None,
+                    chunk_size: int = 64, mask_lmk: bool = True, expand_to_chunk: bool = True, sm_scale: Optional[float] = None,
+                    workspace: Optional[torch.Tensor] = None):
+    """Attention of a tree of drafted tokens per sequence over the paged store (inference only).
+
+    q (B, n, h_q, D), k_new, v_new (B, n, h_kv, D): up to 64 drafted tokens; k_pages, v_pages (num_pages, h_kv, 64, D),
+    page_table (B, max_pages) and lens (B) int32, max_len >= lens on the host, as in decode_step_paged.  parents (B, n) int32
+    on the device: node j's parent, an earlier node or -1 (child of the last cached token); anything else, or an absent
+    ancestor, makes the node absent (a shorter tree in a batch: pad with -2).  Node j stands at position lens[b] + depth; it
+    sees the cached tokens, its ancestors and itself, within window_size positions (None: all; rounded down to whole chunks
+    when expand_to_chunk), landmark positions excepted when mask_lmk, as flex_attn_tl.  The pages are only read: the
+    accepted tokens are written by commit_drafts.
+    Returns o (B, n, h_q, D), lse (B, n, h_q) fp32 (0 and -inf for rows that see nothing) and the workspace for reuse."""
+    if q.dim() != 4 or k_new.dim() != 4 or k_new.shape != v_new.shape or k_new.shape[:2] != q.shape[:2] or k_new.shape[3] != q.shape[3]:
+        raise ValueError(f"tree_attn_paged: q (B,n,h_q,D), k_new and v_new (B,n,h_kv,D), got {tuple(q.shape)}, {tuple(k_new.shape)}, "
+                         f"{tuple(v_new.shape)}")
+    B, n, h_q, D = q.shape
+    h_kv = k_new.shape[2]
+    if k_pages.shape != v_pages.shape or k_pages.dim() != 4 or k_pages.shape[1:] != (h_kv, chunk_size, D):
+        raise ValueError(f"tree_attn_paged: pools {tuple(k_pages.shape)} / {tuple(v_pages.shape)} for {h_kv} heads of {D} in pages of {chunk_size}")
+    if page_table.dim() != 2 or page_table.shape[0] != B or lens.shape != (B,) or parents.shape != (B, n):
+        raise ValueError(f"tree_attn_paged: page_table {tuple(page_table.shape)}, lens {tuple(lens.shape)}, parents {tuple(parents.shape)} "
+                         f"for {B} sequences of {n} nodes")
+    if page_table.dtype != torch.int32 or lens.dtype != torch.int32 or parents.dtype != torch.int32:
+        raise TypeError("tree_attn_paged: page_table, lens and parents must be int32")
+    dt = dtype_code(q)
+    for t in (k_new, v_new, k_pages, v_pages):
+        if t.dtype != q.dtype:
+            raise TypeError(f"tree_attn_paged: q of {q.dtype}, keys or values of {t.dtype}")
+    for t in (q, k_new, v_new, k_pages, v_pages, page_table, lens, parents):
+        if not t.is_contiguous():
+            raise ValueError("tree_attn_paged: tensors must be contiguous")
+    if window_size is not None and window_size < 1:
+        raise ValueError(f"tree_attn_paged: window_size {window_size} (None for the whole cache)")
+    W = 0 if window_size is None else int(window_size)
+    o = torch.empty_like(q)
+    lse = torch.empty((B, n, h_q), dtype=torch.float32, device=q.device)
+    need = query("hils_tree_attn_paged_workspace_bytes", B, n, h_q, h_kv, D, int(max_len), W, dt)
+    if workspace is None or workspace.numel() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    call("hils_tree_attn_paged", ptr(q), ptr(k_new), ptr(v_new), ptr(k_pages), ptr(v_pages), ptr(page_table), page_table.shape[1],
+         k_pages.shape[0], ptr(lens), int(max_len), ptr(parents), ptr(o), ptr(lse), B, n, h_q, h_kv, D, W, int(chunk_size), int(bool(mask_lmk)),
+         int(bool(expand_to_chunk)), 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), dt,
+         ptr(workspace) if workspace.numel() else None, workspace.numel(), stream())
+    return o, lse, workspace
+
+
 # ------------------------------------------------------------------------------------------
 # pages of the paged store
 # ------------------------------------------------------------------------------------------

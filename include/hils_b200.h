@@ -367,6 +367,30 @@ int hils_qk_norm_rope_bwd(const hils_rope_tensor* tensors, int n_tensors, const 
                           size_t workspace_bytes, void* stream);
 size_t hils_qk_norm_rope_bwd_workspace_bytes(int D);
 
+/* ---------------------------------------------------------------------------------------
+ * Attention of a tree of drafted tokens over the paged store (speculative decoding): the sliding-window branch of
+ * hils_decode_step_paged for up to 64 drafted tokens per sequence, or, window_size = 0, attention over the whole cache.
+ * Inference only; no counterpart in the reference, whose decode feeds one token (hils_attention.py:512-547).
+ *   q, o (B, n, h_q, D); k_new, v_new (B, n, h_kv, D) the drafted tokens, read where they are (nothing is written to the
+ *   pages: hils_commit_drafts does that for the accepted ones); k_pages, v_pages, page_table, lens, max_len as in
+ *   hils_decode_step_paged; parents (B, n) int32, device: an earlier node, -1 (child of the last cached token); any other
+ *   value, or an absent ancestor: the node is absent, o = 0 and lse = -inf.  lse (B, n, h_q) fp32, natural logarithm.
+ *   Node j at position t = lens[b] + depth sees the cached tokens and, of the drafted ones, itself and its ancestors, from
+ *   position t - window_size + 1 on (rounded down to its chunk when expand_to_chunk), without the landmark positions
+ *   ((position + 1) % 64 == 0) when mask_lmk; a row that sees nothing gives o = 0, lse = -inf.  What lies in places no row
+ *   sees (behind a sequence's last token, say) may be anything, NaN included.  D 64 or 128, sm_scale > 0.
+ *   workspace: hils_tree_attn_paged_workspace_bytes() (0 when none is needed).  A page outside the pool or the table is
+ *   skipped and reported through hils_take_device_status (8200001, 8200002).
+ * hils_draft_positions: positions (B, n) int32 of the nodes, -1 for absent ones.
+ * ------------------------------------------------------------------------------------- */
+int hils_tree_attn_paged(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages,
+                         const int32_t* page_table, int page_stride, int num_pages, const int32_t* lens, int max_len,
+                         const int32_t* parents, void* o, float* lse, int B, int n, int h_q, int h_kv, int D,
+                         int window_size, int chunk_size, int mask_lmk, int expand_to_chunk, float sm_scale, int dtype,
+                         void* workspace, size_t workspace_bytes, void* stream);
+size_t hils_tree_attn_paged_workspace_bytes(int B, int n, int h_q, int h_kv, int D, int max_len, int window_size, int dtype);
+int hils_draft_positions(const int32_t* parents, const int32_t* lens, int32_t* positions, int B, int n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
