@@ -32,6 +32,7 @@ int take_status_logz_tc();
 int take_status_paged();
 int take_status_pages();
 int take_status_tree();
+int take_status_tree_tc();
 }  // namespace hils
 
 extern "C" int hils_version(void) { return 100; }
@@ -47,9 +48,10 @@ extern "C" int hils_take_device_status(void) {
   const int f = hils::take_status_paged();
   const int g = hils::take_status_pages();
   const int h = hils::take_status_tree();
-  for (const int v : {a, b, c, d, e, f, g, h})
+  const int i = hils::take_status_tree_tc();
+  for (const int v : {a, b, c, d, e, f, g, h, i})
     if (v < 0) return -1;
-  for (const int v : {a, b, c, d, e, f, g, h})
+  for (const int v : {a, b, c, d, e, f, g, h, i})
     if (v != 0) return v;
   return 0;
 }

@@ -242,10 +242,11 @@ static int tree_splits(int64_t ctas, int tiles, int slots) {
   return best;
 }
 
-static TreeParams tree_plan(int B, int n, int h_q, int h_kv, int max_len, int W) {
+static TreeParams tree_plan(int B, int n, int h_q, int h_kv, int max_len, int W, int dtype) {
   TreeParams p = {};
   p.B = B; p.n = n; p.h_q = h_q; p.h_kv = h_kv; p.W = W;
-  p.row_blocks = (int)(((int64_t)n * (h_q / h_kv) + kTreeRows - 1) / kTreeRows);
+  const int rows = dtype == HILS_BF16 ? 128 : kTreeRows;
+  p.row_blocks = (int)(((int64_t)n * (h_q / h_kv) + rows - 1) / rows);
   p.splits = tree_splits((int64_t)B * h_kv * p.row_blocks, tree_tiles(max_len, W), 148 * 2);
   return p;
 }
@@ -262,12 +263,18 @@ int take_status_tree() {
   return v;
 }
 
+int tree_tc_launch(const TreeParams& p, int D, cudaStream_t st);   // tree_attn_tc.cu
+
 template <typename T, int D>
 static int launch_tree(const TreeParams& p, cudaStream_t st) {
-  const size_t smem = tree_smem_floats<D>() * sizeof(float);
-  cudaFuncSetAttribute(tree_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  tree_attn_kernel<T, D><<<dim3((unsigned)(p.row_blocks * p.splits), (unsigned)p.h_kv, (unsigned)p.B), kTreeThreads, smem, st>>>(p);
-  HILS_LAUNCH_CHECK("tree_attn_paged");
+  if constexpr (sizeof(T) == 2) {
+    if (int rc = tree_tc_launch(p, D, st)) return rc;
+  } else {
+    const size_t smem = tree_smem_floats<D>() * sizeof(float);
+    cudaFuncSetAttribute(tree_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    tree_attn_kernel<T, D><<<dim3((unsigned)(p.row_blocks * p.splits), (unsigned)p.h_kv, (unsigned)p.B), kTreeThreads, smem, st>>>(p);
+    HILS_LAUNCH_CHECK("tree_attn_paged");
+  }
   if (p.splits > 1) {
     const int64_t rows = (int64_t)p.B * p.n * p.h_q;
     tree_join_kernel<T, D><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
@@ -295,7 +302,7 @@ static int check_tree(int B, int n, int h_q, int h_kv, int D, int max_len, int w
 
 extern "C" size_t hils_tree_attn_paged_workspace_bytes(int B, int n, int h_q, int h_kv, int D, int max_len, int window_size, int dtype) {
   if (check_tree(B, n, h_q, h_kv, D, max_len, window_size, 64, dtype) || B == 0 || n == 0) return 0;
-  return tree_workspace(tree_plan(B, n, h_q, h_kv, max_len, window_size), D);
+  return tree_workspace(tree_plan(B, n, h_q, h_kv, max_len, window_size, dtype), D);
 }
 
 extern "C" int hils_tree_attn_paged(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages,
@@ -306,12 +313,13 @@ extern "C" int hils_tree_attn_paged(const void* q, const void* k_new, const void
   if (int rc = check_tree(B, n, h_q, h_kv, D, max_len, window_size, chunk_size, dtype)) return rc;
   HILS_REQUIRE(sm_scale > 0.f && sm_scale <= 3.4e38f, "tree_attn_paged: sm_scale must be positive");
   HILS_REQUIRE(page_stride > 0 && num_pages > 0, "tree_attn_paged: bad size");
+  HILS_REQUIRE((int64_t)num_pages * h_kv * 64 <= 0x7fffffff, "tree_attn_paged: a pool of %d pages of %d heads is too large", num_pages, h_kv);
   HILS_REQUIRE((max_len + 63) / 64 <= page_stride, "tree_attn_paged: %d tokens do not fit a page table of %d pages", max_len, page_stride);
   if (B == 0 || n == 0) return HILS_OK;
   HILS_REQUIRE(q && k_new && v_new && k_pages && v_pages && page_table && lens && parents && o && lse, "tree_attn_paged: null pointer");
   HILS_REQUIRE(((((uintptr_t)q) | ((uintptr_t)k_new) | ((uintptr_t)v_new) | ((uintptr_t)k_pages) | ((uintptr_t)v_pages) | ((uintptr_t)o)) & 15) == 0,
                "tree_attn_paged: tensors must be 16-byte aligned");
-  TreeParams p = tree_plan(B, n, h_q, h_kv, max_len, window_size);
+  TreeParams p = tree_plan(B, n, h_q, h_kv, max_len, window_size, dtype);
   const size_t need = tree_workspace(p, D);
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
     set_error("tree_attn_paged: a 16-byte aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);

@@ -160,6 +160,15 @@ def test_whole_cache(hb, dtype, D, B, n, hq, hk, lens, kinds):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("W", [None, 512])
+def test_many_tiles_in_one_share(hb, dtype, D, W):
+    """Enough (sequence, head) pairs that the tiles are not split: a CTA walks up to 26 of them, places reused many times."""
+    _check(hb, _problem(8, 3, 40, 40, D, dtype, [1600, 640, 64, 1500, 0, 321, 129, 1000], ["random", "chain"], seed=D), W)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("W", [1, 2, 37, 64, 65, 128, 512, 100000])
 @pytest.mark.parametrize("mask_lmk,expand", [(True, True), (False, False), (True, False), (False, True)])
 def test_window_edges(hb, dtype, W, mask_lmk, expand):
