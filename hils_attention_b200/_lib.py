@@ -60,6 +60,8 @@ SIGNATURES = {
     "hils_tree_attn_paged": (_I, [_P] * 6 + [_I] * 2 + [_P, _I] + [_P] * 3 + [_I] * 9 + [_F, _I, _P, _SZ, _P]),
     "hils_tree_attn_paged_workspace_bytes": (_SZ, [_I] * 8),
     "hils_draft_positions": (_I, [_P] * 3 + [_I] * 2 + [_P]),
+    "hils_decode_tree_paged": (_I, [_P] * 7 + [_I] * 2 + [_P, _I] + [_P] * 3 + [_I] + [_P] * 2 + [_I] * 10 + [_F, _I, _P, _SZ, _P]),
+    "hils_decode_tree_paged_workspace_bytes": (_SZ, [_I] * 12),
     "hils_copy_pages": (_I, [_P] * 4 + [_I] * 3 + [_I64] * 2 + [_P]),
     "hils_commit_drafts": (_I, [_P] * 5 + [_I] * 2 + [_P] * 2 + [_I] * 6 + [_I64, _I, _P]),
 }
@@ -79,6 +81,7 @@ KERNELS_PER_CALL = {
     "hils_chunk_weights_fwd": 1, "hils_chunk_weights_bwd": 1, "hils_combine_fwd": 1, "hils_combine_bwd": 1,
     "hils_norm_rope_fwd": 1, "hils_norm_rope_bwd": 1, "hils_qk_norm_rope_fwd": 1, "hils_qk_norm_rope_bwd": 2,
     "hils_tree_attn_paged": 2,     # attention, join (one when the tiles are not split)
+    "hils_decode_tree_paged": 6,   # positions, attention, join, key stream, selection + softmax, sparse + combine
     "hils_decode_step_paged": 5,   # append, then as below
     "hils_decode_step": 4,   # window, key stream, selection + inter-chunk softmax, sparse + combine (the 2 copies not counted)
 }

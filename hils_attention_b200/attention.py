@@ -201,6 +201,46 @@ class HiLSAttentionCore(torch.nn.Module):
         o = o.unsqueeze(1)
         return (o, out[1].unsqueeze(1)) if return_indices else o
 
+    def decode_tree_paged(self, q, k, v, lmk_q, store, parents, return_indices: bool = False):
+        """Drafted trees of all sequences against a paged store: q, lmk_q (B, n, h_q, D), k, v (B, n, h_kv, D) with B =
+        store.batch and n as given to store.begin_tree(n); parents (B, n) int32 on the device (ops.tree_attn_paged).  The drafted
+        tokens are kept in the store's draft buffers.  Returns (B, n, h_q, D).  When it is known which nodes are accepted:
+        store.accept_tree(paths), pool_accepted(store) of every layer, store.end_tree().  Inference only."""
+        if not self.enable_prior_query:
+            raise NotImplementedError("decode_tree_paged needs enable_prior_query=True (the pooled chunk keys live in the store)")
+        kd, vd, ld = store.draft(self.layer_idx)
+        if k.shape != kd.shape or q.shape != ld.shape:
+            raise ValueError(f"decode_tree_paged: q {tuple(q.shape)}, k {tuple(k.shape)}; the step in progress wants {tuple(ld.shape)}, {tuple(kd.shape)}")
+        for place, x in ((kd, k), (vd, v), (ld, lmk_q)):
+            place.copy_(x)
+        k_pages, v_pages, table, lens, lmk_k, prior_b = store.step_args(self.layer_idx)
+        max_len = max((store.length(b) for b in store.active_slots()), default=0)
+        out = ops.decode_tree_paged(q.contiguous(), ld, kd, vd, k_pages, v_pages, table, lens, max_len, parents, lmk_k, prior_b, self.topk,
+                                    self.chunk_size, self.hils_sliding_window, self.enable_softmax1, workspace=getattr(self, "_paged_ws", None),
+                                    return_indices=return_indices)
+        self._paged_ws = out[-1]
+        return out[:2] if return_indices else out[0]
+
+    def pool_accepted(self, store, position_embeddings=None):
+        """Pooled keys and prior biases of the chunks that the accepted tokens complete (between store.accept_tree and
+        store.end_tree, for every layer).  position_embeddings = (cos, sin) of the drafted tokens, (B or 1, n, D): only read
+        when the shared prior query is rotated."""
+        slots, nodes = store.completed()
+        if not slots:
+            return
+        layer = self.layer_idx
+        dev = store.k_pages.device
+        rows, cols = (torch.tensor(x, dtype=torch.long, device=dev) for x in (slots, nodes))
+        pe = None
+        if position_embeddings is not None:
+            pe = tuple(x[(rows if x.shape[0] > 1 else torch.zeros_like(rows)), cols].unsqueeze(1) for x in position_embeddings)
+        mu = self._prior_queries(store.draft(layer)[2][rows, cols].unsqueeze(1), slice(0, 1), pe)      # (m, 1, h_q, D)
+        kc = store.chunk_keys(layer, slots).unsqueeze(1)                                               # (m, 1, 64, h_kv, D)
+        new_k, new_b = ops.chunk_attn_pool(mu.contiguous(), kc)
+        if self.enable_chunk_pooling:
+            new_k = ops.chunk_mean_pool(kc)
+        store.put_chunk_keys(layer, slots, new_k[:, 0], new_b[:, 0])
+
     def forward(self, q, k, v, lmk_q, past_key_values=None, use_cache: bool = False,
                 return_aux: bool = False, position_embeddings=None):
         """q, lmk_q (B,L,h_q,D); k, v (B,L,h_kv,D) of the NEW tokens.  Returns (B,L,h_q,Dv), the

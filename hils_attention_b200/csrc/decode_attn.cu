@@ -30,6 +30,7 @@ struct DecodeParams {
   // dtype the chain carries it in.  Sparse kernel: with swa_o given, o = round(o_hils) + w[swa_col] * swa_o, the
   // combination of the two branches with the rounding of the separate kernels.
   void* lse_act; const void* swa_o; int swa_col;
+  const int32_t* row_pos;      // sparse kernel over drafted rows: (B, L), negative: no such row, its output is zero (or null)
 };
 
 // Set when a page table holds an id outside the pool or a chunk past the table's width; the access is skipped.
@@ -212,6 +213,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) sparse_decode_kernel(DecodePar
     if (p.swa_o)
       s = fmaf(to_f(static_cast<const T*>(p.swa_o)[row0 * D + i]), to_f(wts[(i / D) * p.num_weights + p.swa_col]),
                to_f(from_f<T>(s)));
+    if (p.row_pos && p.row_pos[(int64_t)b * p.L + l] < 0) s = 0.f;
     o[i] = from_f<T>(s);
   }
 }
@@ -394,6 +396,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, 2) sparse_decode_bf16_kernel(D
     if (p.swa_o)
       sacc = fmaf(to_f(static_cast<const bf16*>(p.swa_o)[row0 * D + i]), to_f(wts[(i / D) * p.num_weights + p.swa_col]),
                   to_f(__float2bfloat16_rn(sacc)));
+    if (p.row_pos && p.row_pos[(int64_t)b * p.L + l] < 0) sacc = 0.f;
     o[i] = __float2bfloat16_rn(sacc);
   }
 }
@@ -627,6 +630,20 @@ int sparse_decode_paged_launch(const void* q, const void* k_pages, const void* v
   const PagedArgs pa = {pages, lens, page_stride, num_pages, len_add};
   return sparse_decode_impl(q, k_pages, v_pages, w, idx, nullptr, o, B, 1, 0, h_q, h_kv, D, D, K, num_weights, S, scale,
                             mask_last, dtype, st, &pa, swa_o, swa_col);
+}
+
+// The same over the drafted rows of every sequence: lens[b] cached tokens, n rows, row_pos (B, n) their positions.
+int sparse_decode_tree_launch(const void* q, const void* k_pages, const void* v_pages, const void* w, const int32_t* idx,
+                              void* o, const int32_t* pages, const int32_t* lens, const int32_t* row_pos, int page_stride,
+                              int num_pages, int B, int n, int h_q, int h_kv, int D, int K, int num_weights, float scale,
+                              int dtype, cudaStream_t st, const void* swa_o, int swa_col) {
+  DecodeParams p = {};
+  p.q = q; p.k = k_pages; p.v = v_pages; p.w = w; p.idx = idx; p.o = o;
+  p.B = B; p.L = n; p.h_q = h_q; p.h_kv = h_kv; p.D = D; p.K = K; p.num_weights = num_weights; p.S = 64;
+  p.mask_last = 1; p.scale = scale; p.swa_o = swa_o; p.swa_col = swa_col; p.row_pos = row_pos;
+  const PagedArgs pa = {pages, lens, page_stride, num_pages, 0};
+  set_paged(p, &pa);
+  return dtype == HILS_BF16 ? launch_decode<bf16>(p, false, st) : launch_decode<float>(p, false, st);
 }
 
 // The two decode kernels as the one-call decode step uses them over the token-major store: the window kernel also

@@ -67,6 +67,46 @@ int topk_decode_step_launch(const void* q, const void* lmks, const void* lse_swa
                             int h_kv, int G, int D, int topk, int block_size, int window_size, int per_qhead, float sm_scale,
                             int dtype, int lse_dtype, void* workspace, size_t workspace_bytes, cudaStream_t st);
 
+// tree_attn.cu, decode_attn.cu, topk.cu: the stages over drafted rows
+size_t tree_attn_workspace(int B, int n, int h_q, int h_kv, int D, int max_len, int W, int dtype);
+int tree_attn_launch(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                     int page_stride, int num_pages, const int32_t* lens, int max_len, const int32_t* parents, void* o, float* lse,
+                     void* lse_act, int B, int n, int h_q, int h_kv, int D, int W, int mask_lmk, int expand, float scale, int dtype,
+                     void* workspace, size_t workspace_bytes, cudaStream_t st);
+int sparse_decode_tree_launch(const void* q, const void* k_pages, const void* v_pages, const void* w, const int32_t* idx,
+                              void* o, const int32_t* pages, const int32_t* lens, const int32_t* row_pos, int page_stride,
+                              int num_pages, int B, int n, int h_q, int h_kv, int D, int K, int num_weights, float scale,
+                              int dtype, cudaStream_t st, const void* swa_o, int swa_col);
+size_t topk_decode_rows_workspace(int B, int L, int N, int h_kv, int G, int D, int dtype);
+int topk_decode_rows_launch(const void* q, const void* lmks, const void* lse_swa, const float* bias, int32_t* indices,
+                            void* scores, void* weights, int softmax1, const int32_t* q_offsets, const int32_t* row_pos,
+                            int q_offset, int B, int L, int N, int h_kv, int G, int D, int topk, int block_size,
+                            int window_size, int per_qhead, float sm_scale, int dtype, int lse_dtype, void* workspace,
+                            size_t workspace_bytes, cudaStream_t st);
+
+// workspace of the step over drafted trees: the same pieces, per node, the nodes' positions, and what the tree attention wants
+struct TreeStepLayout {
+  StepLayout s;
+  size_t positions, tree_ws, tree_bytes, topk_bytes;
+};
+
+static TreeStepLayout tree_layout(int B, int n, int h_q, int h_kv, int D, int K, int N, int max_len, int W, int softmax1, int dtype) {
+  const size_t es = dtype == HILS_BF16 ? 2 : 4, rows = (size_t)B * n * h_q;
+  TreeStepLayout t;
+  size_t o = 0;
+  t.s.swa_o = o;   o += up256(rows * D * es);
+  t.s.lse32 = o;   o += up256(rows * 4);
+  t.s.lse_act = o; o += up256(rows * es);
+  t.s.scores = o;  o += up256(rows * K * es);
+  t.s.weights = o; o += up256(rows * (K + 1 + (softmax1 ? 1 : 0)) * es);
+  t.s.indices = o; o += up256((size_t)B * n * h_kv * K * 4);
+  t.positions = o; o += up256((size_t)B * n * 4);
+  t.tree_ws = o;   t.tree_bytes = tree_attn_workspace(B, n, h_q, h_kv, D, max_len, W, dtype); o += up256(t.tree_bytes);
+  t.s.topk_ws = o; t.topk_bytes = topk_decode_rows_workspace(B, n, N, h_kv, h_q / h_kv, D, dtype); o += up256(t.topk_bytes);
+  t.s.total = o;
+  return t;
+}
+
 // workspace of the paged step: the same pieces, per sequence
 static StepLayout paged_layout(int B, int h_q, int h_kv, int D, int K, int N, int softmax1, int dtype) {
   const size_t es = dtype == HILS_BF16 ? 2 : 4;
@@ -154,6 +194,72 @@ extern "C" int hils_decode_step_paged(const void* q, const void* lmk_q, const vo
                                             1, B, h_q, h_kv, D, K, nw, chunk_size, sm_scale, 1, dtype, st, swa_o, K);
   if (rc == HILS_ERR_UNSUPPORTED) set_error("decode_step_paged: shape not covered by the decode kernels");
   return rc;
+}
+
+extern "C" size_t hils_decode_tree_paged_workspace_bytes(int B, int n, int h_q, int h_kv, int h_lmk, int D, int K, int N, int max_len,
+                                                         int window_size, int softmax1, int dtype) {
+  if (B <= 0 || n <= 0 || n > 64 || h_kv <= 0 || h_q % h_kv != 0 || (h_lmk != h_kv && h_lmk != h_q) || max_len < 0 || window_size <= 0) return 0;
+  return tree_layout(B, n, h_q, h_kv, D, K, N, max_len, window_size, softmax1, dtype).s.total;
+}
+
+extern "C" int hils_decode_tree_paged(const void* q, const void* lmk_q, const void* k_new, const void* v_new, const void* k_pages,
+                                      const void* v_pages, const int32_t* page_table, int page_stride, int num_pages,
+                                      const int32_t* lens, int max_len, const int32_t* parents, const void* lmk_k, const float* prior_b,
+                                      int N, void* o, int32_t* indices_out, int B, int n, int h_q, int h_kv, int h_lmk, int D, int K,
+                                      int chunk_size, int window_size, int softmax1, float sm_scale, int dtype, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  HILS_REQUIRE(dtype == HILS_BF16 || dtype == HILS_F32, "decode_tree_paged: dtype must be bf16 or fp32");
+  HILS_REQUIRE(B >= 0 && B <= 65535 && n >= 0 && n <= 64, "decode_tree_paged: %d sequences of %d nodes (at most 65535 of 64)", B, n);
+  HILS_REQUIRE(h_q > 0 && h_kv > 0 && h_q % h_kv == 0, "decode_tree_paged: h_q must be a multiple of h_kv");
+  HILS_REQUIRE(h_lmk == h_kv || h_lmk == h_q, "decode_tree_paged: the chunk keys must have h_kv or h_q heads");
+  HILS_REQUIRE(chunk_size == 64, "decode_tree_paged: the page is the chunk and must hold 64 tokens (got %d)", chunk_size);
+  HILS_REQUIRE(D == 64 || D == 128, "decode_tree_paged: head dimension %d (64 or 128)", D);
+  HILS_REQUIRE(K > 0 && K <= 32, "decode_tree_paged: topk %d (1..32)", K);
+  HILS_REQUIRE(h_q / h_kv <= 8 && h_kv <= 65535, "decode_tree_paged: at most 8 query heads per kv head");
+  // a chunk that a node selects ends before its window: with n <= window it ends before the drafted tokens
+  HILS_REQUIRE(window_size >= n, "decode_tree_paged: a window of %d tokens does not hold a tree of %d nodes", window_size, n);
+  HILS_REQUIRE(N > 0 && page_stride > 0 && num_pages > 0 && max_len >= 0 && max_len <= 0x7fffffff - 256, "decode_tree_paged: bad size");
+  HILS_REQUIRE((int64_t)num_pages * h_kv * 64 <= 0x7fffffff, "decode_tree_paged: a pool of %d pages of %d heads is too large", num_pages, h_kv);
+  HILS_REQUIRE((max_len + chunk_size - 1) / chunk_size <= page_stride, "decode_tree_paged: %d tokens do not fit a page table of %d pages",
+               max_len, page_stride);
+  HILS_REQUIRE(max_len / chunk_size <= N, "decode_tree_paged: %d complete chunks but room for %d chunk keys", max_len / chunk_size, N);
+  HILS_REQUIRE((int64_t)B * n * h_q * (N / 1024 + 1) <= 0x7fffffff, "decode_tree_paged: too many rows");
+  HILS_REQUIRE(sm_scale > 0.f && sm_scale <= 3.4e38f, "decode_tree_paged: sm_scale must be positive");
+  if (B == 0 || n == 0) return HILS_OK;
+  HILS_REQUIRE(q && lmk_q && k_new && v_new && k_pages && v_pages && page_table && lens && parents && lmk_k && o, "decode_tree_paged: null pointer");
+  HILS_REQUIRE(((((uintptr_t)q) | ((uintptr_t)k_new) | ((uintptr_t)v_new) | ((uintptr_t)k_pages) | ((uintptr_t)v_pages) | ((uintptr_t)lmk_k) |
+                 ((uintptr_t)lmk_q) | ((uintptr_t)o)) & 15) == 0, "decode_tree_paged: tensors must be 16-byte aligned");
+  const TreeStepLayout lay = tree_layout(B, n, h_q, h_kv, D, K, N, max_len, window_size, softmax1, dtype);
+  if (!workspace || workspace_bytes < lay.s.total || ((uintptr_t)workspace & 15)) {
+    set_error("decode_tree_paged: a 16-byte aligned workspace of %zu bytes needed, %zu given", lay.s.total, workspace_bytes);
+    return HILS_ERR_WORKSPACE;
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  void* swa_o = ws + lay.s.swa_o;
+  void* lse_act = ws + lay.s.lse_act;
+  void* scores = ws + lay.s.scores;
+  void* weights = ws + lay.s.weights;
+  int32_t* positions = reinterpret_cast<int32_t*>(ws + lay.positions);
+  int32_t* indices = indices_out ? indices_out : reinterpret_cast<int32_t*>(ws + lay.s.indices);
+  // 1. positions of the nodes
+  if (int rc = hils_draft_positions(parents, lens, positions, B, n, stream)) return rc;
+  // 2. sliding-window branch: cached tokens of the window, ancestors, the node itself
+  if (int rc = tree_attn_launch(q, k_new, v_new, k_pages, v_pages, page_table, page_stride, num_pages, lens, max_len, parents, swa_o,
+                                reinterpret_cast<float*>(ws + lay.s.lse32), lse_act, B, n, h_q, h_kv, D, window_size, 1, 1, sm_scale, dtype,
+                                ws + lay.tree_ws, lay.tree_bytes, st))
+    return rc;
+  // 3. chunk selection of every node at its own position, then prior-bias gather + softmax over [chunks, window(, 0)]
+  const int nw = K + 1 + (softmax1 ? 1 : 0);
+  if (int rc = topk_decode_rows_launch(lmk_q, lmk_k, lse_act, prior_b, indices, scores, weights, softmax1, nullptr, positions, max_len, B, n, N,
+                                       h_kv, h_q / h_kv, D, K, chunk_size, window_size, h_lmk == h_q && h_q != h_kv, sm_scale, dtype, dtype,
+                                       ws + lay.s.topk_ws, lay.topk_bytes, st)) {
+    if (rc == HILS_ERR_UNSUPPORTED) set_error("decode_tree_paged: selection shape not covered by the decode kernels");
+    return rc;
+  }
+  // 4. sparse chunk attention over the selected pages, and o = o_hils + w_swa * o_swa
+  return sparse_decode_tree_launch(q, k_pages, v_pages, weights, indices, o, page_table, lens, positions, page_stride, num_pages, B, n, h_q,
+                                   h_kv, D, K, nw, sm_scale, dtype, st, swa_o, K);
 }
 
 extern "C" size_t hils_decode_step_workspace_bytes(int heads_q, int heads_kv, int heads_lmk, int D, int K, int N,

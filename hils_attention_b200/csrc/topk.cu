@@ -47,10 +47,11 @@ __host__ __device__ __forceinline__ int row_limit(const TopkParams& p, int l) {
 
 // decode kernels: sequences of one batch may stand at different positions
 __device__ __forceinline__ int row_limit_b(const TopkParams& p, int b, int l) {
-  if (!p.q_offsets) return row_limit(p, l);
+  if (!p.q_offsets && !p.row_pos) return row_limit(p, l);
   if (l >= p.L) return 0;
   if (!p.is_causal) return p.N;
-  const int t = p.q_offsets[b] + l;
+  const int t = p.row_pos ? p.row_pos[(int64_t)b * p.L + l] : p.q_offsets[b] + l;
+  if (p.row_pos && t < 0) return 0;
   const int lim = (p.window_size > 0) ? floor_div(t - p.window_size + 1, p.block_size) : floor_div(t, p.block_size);
   return max(0, min(lim, p.N));
 }
@@ -1411,7 +1412,7 @@ extern "C" int hils_topk_fwd(const void* q, const void* lmks, const void* lse_sw
   p.indices = indices; p.scores = scores; p.lse_total = lse_total; p.rank_keys = rank_keys;
   p.B = B; p.L = L; p.N = N; p.h_kv = h_kv; p.G = G; p.D = D; p.topk = topk; p.block_size = block_size;
   p.window_size = window_size; p.is_causal = is_causal; p.q_offset = q_offset; p.per_qhead = per_qhead;
-  p.lse_dtype = lse_dtype; p.RW = 4; p.scale = sm_scale; p.dots = nullptr; p.q_offsets = nullptr;
+  p.lse_dtype = lse_dtype; p.RW = 4; p.scale = sm_scale; p.dots = nullptr; p.q_offsets = nullptr; p.row_pos = nullptr;
   p.weights = nullptr; p.softmax1 = 0;
   cudaStream_t st = (cudaStream_t)stream;
   // few query rows against many chunk keys (decode, short chunk-prefill): stream the keys once per row
@@ -1446,29 +1447,46 @@ extern "C" int hils_topk_fwd(const void* q, const void* lmks, const void* lse_sw
 }
 
 namespace hils {
-// Selection of the decode step: one new query row per sequence, always on the decode kernels, with the step's
+// Scratch of the decode selection over L rows per sequence: the raw dot products, where the keys are streamed
+size_t topk_decode_rows_workspace(int B, int L, int N, int h_kv, int G, int D, int dtype) {
+  return (size_t)L * hils_topk_fwd_workspace_bytes(B, 1, N, h_kv, G, D, dtype);
+}
+
+// Selection of the decode step: the new query rows of each sequence, always on the decode kernels, with the step's
 // inter-chunk softmax fused behind it (weights, or null).  q_offsets (device, or null) holds each sequence's position
 // when the sequences stand at different ones; q_offset is then the largest of them (host; it sizes the key stream).
+// row_pos (device, (B, L), or null): a position for every row instead (drafted trees; negative: no such row), q_offset + L - 1
+// at least as large as any of them.
 // The chunk keys are (B, N, heads, D) with N the row stride of every sequence; rows at or past a sequence's own limit
 // are never read.  Shapes the decode kernels do not cover are refused (HILS_ERR_UNSUPPORTED).
-int topk_decode_step_launch(const void* q, const void* lmks, const void* lse_swa, const float* bias, int32_t* indices,
-                            void* scores, void* weights, int softmax1, const int32_t* q_offsets, int q_offset, int B, int N,
-                            int h_kv, int G, int D, int topk, int block_size, int window_size, int per_qhead, float sm_scale,
-                            int dtype, int lse_dtype, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+int topk_decode_rows_launch(const void* q, const void* lmks, const void* lse_swa, const float* bias, int32_t* indices,
+                            void* scores, void* weights, int softmax1, const int32_t* q_offsets, const int32_t* row_pos,
+                            int q_offset, int B, int L, int N, int h_kv, int G, int D, int topk, int block_size,
+                            int window_size, int per_qhead, float sm_scale, int dtype, int lse_dtype, void* workspace,
+                            size_t workspace_bytes, cudaStream_t st) {
   if (!(D == 64 || D == 128) || topk > 32 || B > 65535 || h_kv > 65535 || N <= 0) return HILS_ERR_UNSUPPORTED;
   if (weights && lse_dtype != dtype) return HILS_ERR_UNSUPPORTED;
   TopkParams p;
   p.q = q; p.lmks = lmks; p.lse_swa = lse_swa; p.bias = bias; p.gumbel = nullptr; p.drop_mask = nullptr;
   p.indices = indices; p.scores = scores; p.lse_total = nullptr; p.rank_keys = nullptr;
-  p.B = B; p.L = 1; p.N = N; p.h_kv = h_kv; p.G = G; p.D = D; p.topk = topk; p.block_size = block_size;
+  p.B = B; p.L = L; p.N = N; p.h_kv = h_kv; p.G = G; p.D = D; p.topk = topk; p.block_size = block_size;
   p.window_size = window_size; p.is_causal = 1; p.q_offset = q_offset; p.per_qhead = per_qhead;
-  p.lse_dtype = lse_dtype; p.RW = 4; p.scale = sm_scale; p.dots = nullptr; p.q_offsets = q_offsets;
+  p.lse_dtype = lse_dtype; p.RW = 4; p.scale = sm_scale; p.dots = nullptr; p.q_offsets = q_offsets; p.row_pos = row_pos;
   p.weights = weights; p.softmax1 = softmax1;
-  const size_t need = hils_topk_fwd_workspace_bytes(B, 1, N, h_kv, G, D, dtype);
+  const size_t need = topk_decode_rows_workspace(B, L, N, h_kv, G, D, dtype);
   if (workspace && need > 0 && workspace_bytes >= need && (int64_t)B * h_kv <= 65535) p.dots = static_cast<float*>(workspace);
   return (dtype != HILS_BF16) ? launch_topk_decode<float, 0>(p, st)
          : (D == 128)         ? launch_topk_decode<bf16, 8>(p, st)
                               : launch_topk_decode<bf16, 4>(p, st);
+}
+
+int topk_decode_step_launch(const void* q, const void* lmks, const void* lse_swa, const float* bias, int32_t* indices,
+                            void* scores, void* weights, int softmax1, const int32_t* q_offsets, int q_offset, int B, int N,
+                            int h_kv, int G, int D, int topk, int block_size, int window_size, int per_qhead, float sm_scale,
+                            int dtype, int lse_dtype, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  return topk_decode_rows_launch(q, lmks, lse_swa, bias, indices, scores, weights, softmax1, q_offsets, nullptr, q_offset, B, 1, N,
+                                 h_kv, G, D, topk, block_size, window_size, per_qhead, sm_scale, dtype, lse_dtype, workspace,
+                                 workspace_bytes, st);
 }
 }  // namespace hils
 

@@ -15,6 +15,7 @@ struct TopkParams {
   // in the element type, or null: softmax over [scores + bias of the selected chunks, lse_swa(, 0 when softmax1)]
   void* weights; int softmax1;
   const int32_t* q_offsets;   // decode kernels only: position of query row 0 of each batch entry (null: q_offset for all)
+  const int32_t* row_pos;     // decode kernels only: position of every query row (B, L), negative: no such row (null: as above)
 };
 
 }  // namespace hils

@@ -168,7 +168,11 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeParams p) {
       for (int e = 0; e < CPT; e += 4)
         store4(static_cast<T*>(p.o) + out * D + e * 16 + tx * 4,
                make_float4(acc[i][e] * inv, acc[i][e + 1] * inv, acc[i][e + 2] * inv, acc[i][e + 3] * inv));
-      if (tx == 0) p.lse[out] = l > 0.f ? m + logf(l) : (l == l ? -CUDART_INF_F : l);
+      if (tx == 0) {
+        const float lse = l > 0.f ? m + logf(l) : (l == l ? -CUDART_INF_F : l);
+        p.lse[out] = lse;
+        if (p.lse_act) static_cast<T*>(p.lse_act)[out] = from_f<T>(lse);
+      }
     } else {
       const int64_t at = (int64_t)split * p.B * p.n * p.h_q + out;
 #pragma unroll
@@ -212,7 +216,11 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
     o[e * 32 + lane * 2] = from_f<T>(acc[e] * inv);
     o[e * 32 + lane * 2 + 1] = from_f<T>(acc[e + 1] * inv);
   }
-  if (lane == 0) p.lse[row] = l > 0.f ? (ref + log2f(l)) * kLn2F : (l == l ? -CUDART_INF_F : l);
+  if (lane == 0) {
+    const float lse = l > 0.f ? (ref + log2f(l)) * kLn2F : (l == l ? -CUDART_INF_F : l);
+    p.lse[row] = lse;
+    if (p.lse_act) static_cast<T*>(p.lse_act)[row] = from_f<T>(lse);
+  }
 }
 
 // Positions of the nodes, -1 for those that are absent.
@@ -283,6 +291,30 @@ static int launch_tree(const TreeParams& p, cudaStream_t st) {
   return HILS_OK;
 }
 
+size_t tree_attn_workspace(int B, int n, int h_q, int h_kv, int D, int max_len, int W, int dtype) {
+  return tree_workspace(tree_plan(B, n, h_q, h_kv, max_len, W, dtype), D);
+}
+
+// Checked arguments; lse_act as in TreeParams.
+int tree_attn_launch(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                     int page_stride, int num_pages, const int32_t* lens, int max_len, const int32_t* parents, void* o, float* lse,
+                     void* lse_act, int B, int n, int h_q, int h_kv, int D, int W, int mask_lmk, int expand, float scale, int dtype,
+                     void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  TreeParams p = tree_plan(B, n, h_q, h_kv, max_len, W, dtype);
+  const size_t need = tree_workspace(p, D);
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
+    set_error("tree_attn_paged: a 16-byte aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    return HILS_ERR_WORKSPACE;
+  }
+  p.q = q; p.k_new = k_new; p.v_new = v_new; p.k_pages = k_pages; p.v_pages = v_pages; p.pages = page_table; p.lens = lens;
+  p.parents = parents; p.o = o; p.lse = lse; p.lse_act = lse_act; p.page_stride = page_stride; p.num_pages = num_pages;
+  p.mask_lmk = mask_lmk; p.expand = expand; p.scale = scale;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + (size_t)p.splits * B * n * h_q * D;
+  if (dtype == HILS_BF16) return D == 128 ? launch_tree<bf16, 128>(p, st) : launch_tree<bf16, 64>(p, st);
+  return D == 128 ? launch_tree<float, 128>(p, st) : launch_tree<float, 64>(p, st);
+}
+
 }  // namespace hils
 
 using namespace hils;
@@ -302,7 +334,7 @@ static int check_tree(int B, int n, int h_q, int h_kv, int D, int max_len, int w
 
 extern "C" size_t hils_tree_attn_paged_workspace_bytes(int B, int n, int h_q, int h_kv, int D, int max_len, int window_size, int dtype) {
   if (check_tree(B, n, h_q, h_kv, D, max_len, window_size, 64, dtype) || B == 0 || n == 0) return 0;
-  return tree_workspace(tree_plan(B, n, h_q, h_kv, max_len, window_size, dtype), D);
+  return tree_attn_workspace(B, n, h_q, h_kv, D, max_len, window_size, dtype);
 }
 
 extern "C" int hils_tree_attn_paged(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages,
@@ -319,20 +351,9 @@ extern "C" int hils_tree_attn_paged(const void* q, const void* k_new, const void
   HILS_REQUIRE(q && k_new && v_new && k_pages && v_pages && page_table && lens && parents && o && lse, "tree_attn_paged: null pointer");
   HILS_REQUIRE(((((uintptr_t)q) | ((uintptr_t)k_new) | ((uintptr_t)v_new) | ((uintptr_t)k_pages) | ((uintptr_t)v_pages) | ((uintptr_t)o)) & 15) == 0,
                "tree_attn_paged: tensors must be 16-byte aligned");
-  TreeParams p = tree_plan(B, n, h_q, h_kv, max_len, window_size, dtype);
-  const size_t need = tree_workspace(p, D);
-  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
-    set_error("tree_attn_paged: a 16-byte aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
-    return HILS_ERR_WORKSPACE;
-  }
-  p.q = q; p.k_new = k_new; p.v_new = v_new; p.k_pages = k_pages; p.v_pages = v_pages; p.pages = page_table; p.lens = lens;
-  p.parents = parents; p.o = o; p.lse = lse; p.page_stride = page_stride; p.num_pages = num_pages;
-  p.mask_lmk = mask_lmk; p.expand = expand_to_chunk; p.scale = sm_scale;
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + (size_t)p.splits * B * n * h_q * D;
-  cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == HILS_BF16) return D == 128 ? launch_tree<bf16, 128>(p, st) : launch_tree<bf16, 64>(p, st);
-  return D == 128 ? launch_tree<float, 128>(p, st) : launch_tree<float, 64>(p, st);
+  return hils::tree_attn_launch(q, k_new, v_new, k_pages, v_pages, page_table, page_stride, num_pages, lens, max_len, parents, o, lse, nullptr, B,
+                                n, h_q, h_kv, D, window_size, mask_lmk, expand_to_chunk, sm_scale, dtype, workspace, workspace_bytes,
+                                (cudaStream_t)stream);
 }
 
 extern "C" int hils_draft_positions(const int32_t* parents, const int32_t* lens, int32_t* positions, int B, int n, void* stream) {

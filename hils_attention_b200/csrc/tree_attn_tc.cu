@@ -404,7 +404,9 @@ __global__ void __launch_bounds__(kTtThreads, 2) tree_attn_tc_kernel(const __gri
       if (p.splits > 1) {
         *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, have ? l : 0.f);
       } else {
-        p.lse[out] = l > 0.f ? (m + log2f(l)) * kLn2F : (l == l ? -CUDART_INF_F : l);
+        const float lse = l > 0.f ? (m + log2f(l)) * kLn2F : (l == l ? -CUDART_INF_F : l);
+        p.lse[out] = lse;
+        if (p.lse_act) static_cast<bf16*>(p.lse_act)[out] = __float2bfloat16_rn(lse);
       }
     }
   }

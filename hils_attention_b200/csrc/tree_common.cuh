@@ -21,6 +21,7 @@ struct TreeParams {
   const void* q; const void* k_new; const void* v_new; const void* k_pages; const void* v_pages;
   const int32_t* pages; const int32_t* lens; const int32_t* parents;
   void* o; float* lse;
+  void* lse_act;                       // or null: lse again, rounded to the activation type
   float* part_o; float* part_ml;       // splits > 1: (split, b, node, head) rows of D unnormalised sums, and (log2 max, sum)
   int B, n, h_q, h_kv, W, mask_lmk, expand, page_stride, num_pages, splits, row_blocks;
   float scale;

@@ -16,7 +16,8 @@ store - are kept dense per sequence slot, since the selection streams all of the
 
 Full pages are never written again, so several sequences may share them: `fork` gives a second sequence the pages of the
 first (a reference count per page, only the unfinished last page is copied), `compact` moves the pages in use to the front of
-the pool.
+the pool.  A step over a tree of drafted tokens (`begin_tree` .. `end_tree`) keeps the drafts beside the pages until it is
+known which of them are accepted; only those are written.
 
 Host-side bookkeeping (free list, tables, lengths) is plain Python and mirrors what sits on the device;
 nothing here reads device memory back, so a decode step issues no synchronisation.
@@ -134,6 +135,9 @@ class PagedKVStore:
         self._lens: List[int] = [0] * max_seqs
         self._active: List[bool] = [False] * max_seqs
         self._in_step = False
+        self._tree = 0                                              # nodes per sequence of the drafted step in progress
+        self._drafts: Optional[Tuple[torch.Tensor, ...]] = None     # k, v, lmk_q of the drafted tokens of every layer
+        self._paths: Optional[List[List[int]]] = None               # accepted nodes per slot, between accept_tree and end_tree
 
     # ---- bookkeeping ---------------------------------------------------------------------------------
     @property
@@ -334,7 +338,7 @@ class PagedKVStore:
 
     def end_step(self) -> None:
         """Every active sequence is one token longer (after all layers ran the step)."""
-        if not self._in_step:
+        if not self._in_step or self._tree:
             raise RuntimeError("end_step() without begin_step()")
         n = self.batch
         self.lens[:n].add_(self._active_dev[:n])
@@ -342,6 +346,71 @@ class PagedKVStore:
             if self._active[b]:
                 self._lens[b] += 1
         self._in_step = False
+
+    # ---- a step over drafted trees -------------------------------------------------------------------
+    def begin_tree(self, n: int) -> int:
+        """Begin a step over trees of up to `n` drafted tokens per sequence (at most 64) and return max_len.  Every active
+        sequence gets the pages for n more tokens; unused ones stay reserved for its next tokens."""
+        if self._in_step:
+            raise RuntimeError("begin_tree() between begin_step() / begin_tree() and its end")
+        if not 1 <= n <= 64:
+            raise ValueError(f"a tree of {n} nodes (1 to 64)")
+        self._reserve({b: n for b in self.active_slots()})
+        shape = (self.num_layers, self.batch, n)
+        if self._drafts is None or self._drafts[0].shape[:3] != shape:
+            self._drafts = tuple(torch.empty((*shape, h, self.D), dtype=self.dtype, device=self.device) for h in (self.h_kv, self.h_kv, self.h_q))
+        self._in_step, self._tree, self._paths = True, int(n), None
+        return max((self._lens[b] for b in self.active_slots()), default=0)
+
+    def draft(self, layer: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """The places of the drafted tokens of one layer in the step in progress: k, v (batch, n, h_kv, D) and the landmark
+        query (batch, n, h_q, D), which the pooled key of a chunk completed by an accepted token needs."""
+        if not self._tree:
+            raise RuntimeError("draft() without begin_tree()")
+        return tuple(t[layer] for t in self._drafts)
+
+    def accept_tree(self, paths: Sequence[Sequence[int]]) -> None:
+        """After all layers ran: the nodes to keep of every row of the batch, from the root of the accepted path on (node ids
+        ascend along a path; empty: nothing accepted).  Their keys and values are written into the pages."""
+        if not self._tree or self._paths is not None:
+            raise RuntimeError("accept_tree() once per begin_tree()")
+        paths = [[int(x) for x in p] for p in paths]
+        if len(paths) != self.batch:
+            raise ValueError(f"accept_tree: {len(paths)} paths for a batch of {self.batch}")
+        for b, p in enumerate(paths):
+            if any(not 0 <= x < self._tree for x in p) or any(x >= y for x, y in zip(p, p[1:])):
+                raise ValueError(f"accept_tree: path {p} of slot {b} is not an ascending list of nodes below {self._tree}")
+            if p and not self._active[b]:
+                raise ValueError(f"accept_tree: slot {b} is not active")
+        width = max((len(p) for p in paths), default=0)
+        if width:
+            t = torch.tensor([p + [-1] * (width - len(p)) for p in paths], dtype=torch.int32).to(self.device, non_blocking=True)
+            self._commit_drafts(t)
+        self._paths = paths
+
+    def _commit_drafts(self, path: torch.Tensor) -> None:
+        n = self.batch
+        k, v, _ = self._drafts
+        ops.commit_drafts(k, v, self.k_pages, self.v_pages, self.page_table[:n], self.lens[:n], path)
+
+    def completed(self) -> Tuple[List[int], List[int]]:
+        """Slots whose chunk the accepted tokens complete, and the node that is the chunk's last token (at most one chunk per
+        sequence: a tree has at most 64 nodes)."""
+        if self._paths is None:
+            raise RuntimeError("completed() before accept_tree()")
+        slots = [b for b, p in enumerate(self._paths) if self._lens[b] % self.S + len(p) >= self.S]
+        return slots, [self._paths[b][self.S - 1 - self._lens[b] % self.S] for b in slots]
+
+    def end_tree(self) -> None:
+        """Every sequence is longer by its accepted path (after the chunks these tokens complete got their pooled keys)."""
+        if self._paths is None:
+            raise RuntimeError("end_tree() before accept_tree()")
+        n = self.batch
+        if n:
+            self.lens[:n].add_(torch.tensor([len(p) for p in self._paths], dtype=torch.int32).to(self.device, non_blocking=True))
+        for b, p in enumerate(self._paths):
+            self._lens[b] += len(p)
+        self._in_step, self._tree, self._paths = False, 0, None
 
     def bytes_held(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k_pages, self.v_pages, self.lmk_k, self.prior_b,

@@ -569,6 +569,53 @@ def tree_attn_paged(q, k_new, v_new, k_pages, v_pages, page_table, lens, max_len
     return o, lse, workspace
 
 
+def decode_tree_paged(q, lmk_q, k_new, v_new, k_pages, v_pages, page_table, lens, max_len: int, parents, lmk_k, prior_b, topk: int,
+                      chunk_size: int = 64, window_size: int = 512, softmax1: bool = False, sm_scale: Optional[float] = None,
+                      workspace: Optional[torch.Tensor] = None, return_indices: bool = False):
+    """The decode step of `decode_step_paged` for a tree of drafted tokens per sequence, in one library call (inference only).
+
+    q, lmk_q (B, n, h_q, D), k_new, v_new (B, n, h_kv, D), parents (B, n) int32 as in `tree_attn_paged` (the window branch);
+    every node selects its chunks and attends to them at its own position.  n <= 64 and n <= window_size.  The pages and
+    lens are left as they are: `commit_drafts` writes the accepted nodes.
+    Returns o (B, n, h_q, D) (zeros for absent nodes) [, indices (B, n, h_kv, topk)] and the workspace for reuse."""
+    if q.dim() != 4 or lmk_q.shape != q.shape or k_new.dim() != 4 or k_new.shape != v_new.shape or k_new.shape[:2] != q.shape[:2]:
+        raise ValueError(f"decode_tree_paged: q, lmk_q (B,n,h_q,D), k_new, v_new (B,n,h_kv,D), got {tuple(q.shape)}, {tuple(lmk_q.shape)}, "
+                         f"{tuple(k_new.shape)}, {tuple(v_new.shape)}")
+    B, n, h_q, D = q.shape
+    h_kv = k_new.shape[2]
+    if k_pages.shape != v_pages.shape or k_pages.dim() != 4 or k_pages.shape[1:] != (h_kv, chunk_size, D) or k_new.shape[3] != D:
+        raise ValueError(f"decode_tree_paged: pools {tuple(k_pages.shape)} / {tuple(v_pages.shape)} for {h_kv} heads of {D} in pages of {chunk_size}")
+    if page_table.dim() != 2 or page_table.shape[0] != B or lens.shape != (B,) or parents.shape != (B, n):
+        raise ValueError(f"decode_tree_paged: page_table {tuple(page_table.shape)}, lens {tuple(lens.shape)}, parents {tuple(parents.shape)} "
+                         f"for {B} sequences of {n} nodes")
+    if lmk_k.dim() != 4 or lmk_k.shape[0] != B or lmk_k.shape[3] != D:
+        raise ValueError(f"decode_tree_paged: chunk keys {tuple(lmk_k.shape)} for {B} sequences of heads of {D}")
+    N, h_lmk = lmk_k.shape[1], lmk_k.shape[2]
+    if page_table.dtype != torch.int32 or lens.dtype != torch.int32 or parents.dtype != torch.int32:
+        raise TypeError("decode_tree_paged: page_table, lens and parents must be int32")
+    dt = dtype_code(q)
+    for t in (lmk_q, k_new, v_new, k_pages, v_pages, lmk_k):
+        if t.dtype != q.dtype:
+            raise TypeError(f"decode_tree_paged: q of {q.dtype}, another tensor of {t.dtype}")
+    for t in (q, lmk_q, k_new, v_new, k_pages, v_pages, page_table, lens, parents, lmk_k):
+        if not t.is_contiguous():
+            raise ValueError("decode_tree_paged: tensors must be contiguous")
+    pb = None if prior_b is None else prior_b.to(torch.float32).contiguous()
+    if pb is not None and pb.shape != (B, N, h_q):
+        raise ValueError(f"decode_tree_paged: prior_b {tuple(pb.shape)}, expected {(B, N, h_q)}")
+    o = torch.empty_like(q)
+    idx = torch.empty((B, n, h_kv, topk), dtype=torch.int32, device=q.device) if return_indices else None
+    need = query("hils_decode_tree_paged_workspace_bytes", B, n, h_q, h_kv, h_lmk, D, int(topk), N, int(max_len), int(window_size),
+                 int(bool(softmax1)), dt)
+    if workspace is None or workspace.numel() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    call("hils_decode_tree_paged", ptr(q), ptr(lmk_q), ptr(k_new), ptr(v_new), ptr(k_pages), ptr(v_pages), ptr(page_table), page_table.shape[1],
+         k_pages.shape[0], ptr(lens), int(max_len), ptr(parents), ptr(lmk_k), ptr(pb), N, ptr(o), ptr(idx), B, n, h_q, h_kv, h_lmk, D, int(topk),
+         int(chunk_size), int(window_size), int(bool(softmax1)), 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), dt,
+         ptr(workspace) if workspace.numel() else None, workspace.numel(), stream())
+    return (o, idx, workspace) if return_indices else (o, workspace)
+
+
 # ------------------------------------------------------------------------------------------
 # pages of the paged store
 # ------------------------------------------------------------------------------------------

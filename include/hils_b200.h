@@ -391,6 +391,19 @@ int hils_tree_attn_paged(const void* q, const void* k_new, const void* v_new, co
 size_t hils_tree_attn_paged_workspace_bytes(int B, int n, int h_q, int h_kv, int D, int max_len, int window_size, int dtype);
 int hils_draft_positions(const int32_t* parents, const int32_t* lens, int32_t* positions, int B, int n, void* stream);
 
+/* hils_decode_tree_paged: the decode step of hils_decode_step_paged for a tree of drafted tokens per sequence (the tree
+ *   attention as the window branch, selection and sparse chunk attention for every node at its own position).  Arguments as
+ *   there with q, lmk_q, o (B, n, h_q, D), k_new, v_new (B, n, h_kv, D), parents (B, n), indices_out (B, n, h_kv, K) or
+ *   NULL; the pages are only read; n <= window_size; lens is not advanced.  Absent nodes give o = 0. */
+int hils_decode_tree_paged(const void* q, const void* lmk_q, const void* k_new, const void* v_new, const void* k_pages,
+                           const void* v_pages, const int32_t* page_table, int page_stride, int num_pages,
+                           const int32_t* lens, int max_len, const int32_t* parents, const void* lmk_k,
+                           const float* prior_b, int N, void* o, int32_t* indices_out, int B, int n, int h_q, int h_kv,
+                           int h_lmk, int D, int K, int chunk_size, int window_size, int softmax1, float sm_scale,
+                           int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t hils_decode_tree_paged_workspace_bytes(int B, int n, int h_q, int h_kv, int h_lmk, int D, int K, int N, int max_len,
+                                              int window_size, int softmax1, int dtype);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,160 @@
+"""Bookkeeping of a step over drafted trees on CPU tensors (the row writes replaced by plain indexing), and the argument
+checks of the one-call step (no GPU needed)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from hils_attention_b200 import _lib, ops
+from hils_attention_b200.kv_store import PagedKVStore
+
+BAD_ARG, WORKSPACE = -1, -4
+
+
+class _Store(PagedKVStore):
+    def _copy_pages(self, src, dst):
+        self.k_pages[:, list(dst)], self.v_pages[:, list(dst)] = self.k_pages[:, list(src)], self.v_pages[:, list(src)]
+
+    def _commit_drafts(self, path):
+        k, v, _ = self._drafts
+        for b, nodes in enumerate(path.tolist()):
+            for i, x in enumerate(n for n in nodes if n >= 0):
+                t = int(self.lens[b]) + i
+                pg = int(self.page_table[b, t // 64])
+                self.k_pages[:, pg, :, t % 64], self.v_pages[:, pg, :, t % 64] = k[:, b, x], v[:, b, x]
+
+
+def _store(num_pages=12, max_seqs=3, max_pages=4):
+    return _Store(num_pages, max_seqs, max_pages, h_kv=2, head_dim=8, h_q=4, dtype=torch.float32, device="cpu", num_layers=2)
+
+
+def _fill(st):
+    for layer in range(st.num_layers):
+        for t in st.draft(layer):
+            t.copy_(torch.randn(t.shape))
+
+
+def test_accepted_nodes_become_tokens():
+    st = _store()
+    a, b, c = st.allocate(60), st.allocate(0), st.allocate(64)
+    st.release(b)
+    assert st.begin_tree(7) == 64
+    assert [len(st.pages_of(x)) for x in (a, b, c)] == [2, 0, 2]
+    _fill(st)
+    st.accept_tree([[0, 2, 3, 5], [], [1]])
+    assert st.completed() == ([a], [5])                        # a: 60 + 4 tokens; the fourth is node 5
+    kc = st.chunk_keys(0, [a])
+    assert kc.shape == (1, 64, 2, 8) and torch.equal(kc[0, 60:], st.draft(0)[0][a, [0, 2, 3, 5]])
+    st.put_chunk_keys(0, [a], torch.ones(1, 4, 8), torch.ones(1, 4))
+    k1, v1, _ = (t.clone() for t in st.draft(1))
+    st.end_tree()
+    assert (st.length(a), st.length(b), st.length(c)) == (64, 0, 65) and st.lens.tolist() == [64, 0, 65]
+    assert bool((st.lmk_k[0, a, 0] == 1).all())
+    gk, gv = st.gather(c, 1)
+    assert torch.equal(gk[64], k1[c, 1]) and torch.equal(gv[64], v1[c, 1])
+
+
+def test_reserved_pages_are_used_before_new_ones():
+    st = _store()
+    a = st.allocate(63)
+    st.begin_tree(64)                                          # room for 127 tokens
+    assert len(st.pages_of(a)) == 2
+    _fill(st)
+    st.accept_tree([[4]])
+    assert st.completed() == ([a], [4])
+    st.end_tree()
+    free, pages = st.pool.free, st.pages_of(a)
+    st.begin_step()                                            # token 64 goes into the page that is there
+    assert st.pool.free == free and st.pages_of(a) == pages and st.length(a) == 64
+    st.end_step()
+    (b,) = st.fork(a)                                          # a fork shares what is full, not what is reserved
+    assert st.pages_of(b)[0] == pages[0] and len(st.pages_of(b)) == 2 and st.pages_of(b)[1] != pages[1]
+    st.release(a), st.release(b)
+    assert st.pool.free == 11
+
+
+def test_nothing_accepted_and_a_full_tree():
+    st = _store()
+    a = st.allocate(64)
+    st.begin_tree(64)
+    st.accept_tree([[]])
+    assert st.completed() == ([], [])
+    st.end_tree()
+    assert st.length(a) == 64
+    st.begin_tree(64)
+    _fill(st)
+    st.accept_tree([list(range(64))])
+    assert st.completed() == ([a], [63])
+    st.end_tree()
+    assert st.length(a) == 128
+
+
+def test_order_of_calls_and_bad_paths():
+    st = _store(max_pages=2, num_pages=4)
+    a = st.allocate(100)
+    for bad in (0, 65):
+        with pytest.raises(ValueError):
+            st.begin_tree(bad)
+    with pytest.raises(MemoryError):
+        st.begin_tree(29)                                      # 129 tokens, two pages
+    with pytest.raises(RuntimeError):
+        st.draft(0)
+    st.begin_tree(28)
+    for call in (lambda: st.begin_tree(1), st.begin_step, st.end_step, st.end_tree, st.completed, lambda: st.fork(a), st.compact, lambda: st.release(a)):
+        with pytest.raises(RuntimeError):
+            call()
+    for paths in ([], [[0], [1]], [[28]], [[-1]], [[1, 1]], [[2, 1]]):
+        with pytest.raises(ValueError):
+            st.accept_tree(paths)
+    st.accept_tree([[0, 27]])
+    with pytest.raises(RuntimeError):
+        st.accept_tree([[0]])
+    st.end_tree()
+    assert st.length(a) == 102
+    # a path for a row that is no sequence
+    b = st.allocate(0)
+    c = None
+    st2 = _store()
+    x, y = st2.allocate(3), st2.allocate(3)
+    st2.release(x)
+    st2.begin_tree(4)
+    with pytest.raises(ValueError):
+        st2.accept_tree([[0], [1]])
+    st2.accept_tree([[], [1]])
+
+
+def _call(*, B=2, n=8, h_q=4, h_kv=2, h_lmk=4, D=64, K=4, N=16, W=128, S=64, stride=20, pages=90, max_len=1000, scale=0.125, dtype=_lib.BF16, ptr=0x1000,
+          ws=None, ws_bytes=0):
+    lib = _lib.load()
+    p = C.c_void_p(ptr)
+    rc = lib.hils_decode_tree_paged(p, p, p, p, p, p, p, stride, pages, p, max_len, p, p, None, N, p, None, B, n, h_q, h_kv, h_lmk, D, K, S, W, 0, scale,
+                                    dtype, ws, ws_bytes, None)
+    return rc, lib.hils_last_error().decode()
+
+
+def test_the_one_call_step_refuses_bad_arguments():
+    for kw, word in ((dict(n=65, W=512), "nodes"), (dict(n=-1), "nodes"), (dict(B=-1), "sequences"), (dict(h_q=5, h_lmk=5), "multiple"), (dict(h_lmk=3), "chunk keys"),
+                     (dict(S=32), "64 tokens"), (dict(D=96), "head dimension"), (dict(K=33), "topk"), (dict(K=0), "topk"), (dict(h_q=32, h_lmk=32), "8 query heads"),
+                     (dict(W=7), "does not hold"), (dict(N=0), "bad size"), (dict(stride=15), "page table"), (dict(N=14), "chunk keys"), (dict(scale=0.0), "sm_scale"),
+                     (dict(dtype=9), "dtype"), (dict(ptr=0), "null"), (dict(ptr=0x1008), "aligned"), (dict(max_len=-1), "bad size")):
+        rc, err = _call(**kw)
+        assert rc == BAD_ARG and word in err, (kw, err)
+    need = _lib.load().hils_decode_tree_paged_workspace_bytes(2, 8, 4, 2, 4, 64, 4, 16, 1000, 128, 0, _lib.BF16)
+    assert need > 0 and need % 256 == 0
+    for ws, size in ((None, 0), (C.c_void_p(0x2000), need - 1), (C.c_void_p(0x2008), need)):
+        assert _call(ws=ws, ws_bytes=size)[0] == WORKSPACE
+    assert _call(B=0)[0] == 0 and _call(n=0)[0] == 0
+
+
+def test_shapes_and_types_are_refused():
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    ok = dict(q=torch.zeros(2, 3, 4, 64), lmk_q=torch.zeros(2, 3, 4, 64), k_new=torch.zeros(2, 3, 2, 64), v_new=torch.zeros(2, 3, 2, 64),
+              k_pages=torch.zeros(5, 2, 64, 64), v_pages=torch.zeros(5, 2, 64, 64), page_table=i32(2, 4), lens=i32(2), max_len=100, parents=i32(2, 3),
+              lmk_k=torch.zeros(2, 4, 4, 64), prior_b=None, topk=4)
+    for change, err in ((dict(lmk_q=torch.zeros(2, 3, 2, 64)), ValueError), (dict(k_new=torch.zeros(2, 4, 2, 64)), ValueError), (dict(lens=i32(3)), ValueError),
+                        (dict(lmk_k=torch.zeros(3, 4, 4, 64)), ValueError), (dict(prior_b=torch.zeros(2, 4, 2)), ValueError), (dict(parents=i32(2, 3).long()), TypeError),
+                        (dict(lmk_k=torch.zeros(2, 4, 4, 64).bfloat16()), TypeError), (dict(q=torch.zeros(2, 4, 3, 64).transpose(1, 2)), ValueError)):
+        with pytest.raises(err):
+            ops.decode_tree_paged(**{**ok, **change})
+    with pytest.raises(RuntimeError):
+        ops.decode_tree_paged(**ok)                            # not on a GPU
