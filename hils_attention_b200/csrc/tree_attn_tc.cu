@@ -27,12 +27,15 @@ static __device__ int g_tree_tc_expired = 0;
 
 using namespace umma;
 
-constexpr int kTtThreads = 192;           // 4 row warps, 1 that issues the products, 1 that brings the tiles
 constexpr float kTtSlack = 8.f;              // log2 units a row's maximum may grow before O is rescaled
 
-template <int D> struct TtShape {
-  static constexpr int DB = D / 64, QBYTES = DB * 16384, TBYTES = DB * 8192, NS = D == 128 ? 2 : 4;
-  static constexpr int PAT = QBYTES + 2 * NS * TBYTES, BARS = PAT + 16384, SMEM = BARS + 512;
+// TG groups of 128 rows share the tiles of a CTA.  One group: two CTAs per SM, each with places for two tiles of D = 128.
+// Two groups (more than 128 rows per key head): one CTA per SM, every tile is brought once for 256 rows, four places.
+template <int D, int TG> struct TtShape {
+  static constexpr int DB = D / 64, QBYTES = DB * 16384, TBYTES = DB * 8192;
+  static constexpr int NS = TG == 1 ? (D == 128 ? 2 : 4) : (D == 128 ? 4 : 6);
+  static constexpr int THREADS = 128 * TG + 64;            // row warps, one warp that issues the products, one that brings the tiles
+  static constexpr int PAT = TG * QBYTES + 2 * NS * TBYTES, BARS = PAT + TG * 16384, SMEM = BARS + 512;
 };
 
 __device__ __forceinline__ bool not_finite8(uint4 x) {     // eight bf16: an exponent of all ones
@@ -73,25 +76,27 @@ __device__ __forceinline__ void add_bad_keys(const TreeParams& p, const u64t* ba
   }
 }
 
-template <int D>
-__global__ void __launch_bounds__(kTtThreads, 2) tree_attn_tc_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
+template <int D, int TG>
+__global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree_attn_tc_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
                                                                      const __grid_constant__ CUtensorMap tmV) {
-  using Sh = TtShape<D>;
-  constexpr int NS = Sh::NS, DB = Sh::DB, TB = Sh::TBYTES;
+  using Sh = TtShape<D, TG>;
+  constexpr int NS = Sh::NS, DB = Sh::DB, TB = Sh::TBYTES, QB = Sh::QBYTES, kRows = 128 * TG, kThreads = Sh::THREADS;
+  constexpr int kMmaWarp = 4 * TG, kLoadWarp = 4 * TG + 1, kTmem = TG == 1 ? 256 : 512;
   extern __shared__ uint8_t tt_smem[];
   uint8_t* Qs = tt_smem;
-  uint8_t* Ks = Qs + Sh::QBYTES;
+  uint8_t* Ks = Qs + TG * QB;
   uint8_t* Vs = Ks + NS * TB;
   uint8_t* Ps = tt_smem + Sh::PAT;
   uint64_t* bars = reinterpret_cast<uint64_t*>(tt_smem + Sh::BARS);
   uint64_t* k_full = bars;                 // [NS]
   uint64_t* k_free = bars + NS;            // [NS]
   uint64_t* v_full = bars + 2 * NS;        // [NS]
-  uint64_t* v_free = bars + 3 * NS;        // [NS]  also: the product into O is done
-  uint64_t* s_full = bars + 4 * NS;        // [2]
-  uint64_t* p_full = s_full + 2;           // [1]
-  uint64_t* done = p_full + 1;             // [1]
-  u64t* bad_s = reinterpret_cast<u64t*>(done + 1);                   // [3] keys with non-finite values: drafts, tiles c0, c0 + 1
+  uint64_t* v_free = bars + 3 * NS;        // [NS]
+  uint64_t* s_full = bars + 4 * NS;        // [TG][2]
+  uint64_t* p_full = s_full + 2 * TG;      // [TG]
+  uint64_t* pv_done = p_full + TG;         // [TG]
+  uint64_t* done = pv_done + TG;           // [1]
+  u64t* bad_s = reinterpret_cast<u64t*>(done + 1);   // [3] keys with non-finite values: drafts, tiles c0, c0 + 1
   volatile int* tile_ok = reinterpret_cast<volatile int*>(bad_s + 3);   // [8]
   uint32_t& tmem_base_s = *reinterpret_cast<uint32_t*>(const_cast<int*>(tile_ok) + 8);
   volatile int& abort_s = const_cast<volatile int*>(tile_ok)[9];
@@ -110,16 +115,19 @@ __global__ void __launch_bounds__(kTtThreads, 2) tree_attn_tc_kernel(const __gri
       mbar_init(&v_full[s], 1);
       mbar_init(&v_free[s], 1);
     }
-    mbar_init(&s_full[0], 1);
-    mbar_init(&s_full[1], 1);
-    mbar_init(p_full, 128);
+    for (int g = 0; g < TG; ++g) {
+      mbar_init(&s_full[2 * g], 1);
+      mbar_init(&s_full[2 * g + 1], 1);
+      mbar_init(&p_full[g], 128);
+      mbar_init(&pv_done[g], 1);
+    }
     mbar_init(done, 1);
     mbar_init_fence();
     abort_s = *const_cast<volatile int*>(&g_tree_tc_expired) != 0;
     lo_max_s = 0;
     bad_s[0] = bad_s[1] = bad_s[2] = 0ull;
   }
-  if (warp == 4) tmem_alloc(&tmem_base_s, 256);
+  if (warp == kMmaWarp) tmem_alloc(&tmem_base_s, kTmem);
   bool over;
   const int len = tree_length(p, b, over);
   if (over && tid == 0) atomicExch(&g_tree_tc_status, 8200002);
@@ -132,16 +140,16 @@ __global__ void __launch_bounds__(kTtThreads, 2) tree_attn_tc_kernel(const __gri
   int (*par)[kTreeMaxNodes] = reinterpret_cast<int (*)[kTreeMaxNodes]>(Ps);
   u64t (*anc)[kTreeMaxNodes] = reinterpret_cast<u64t (*)[kTreeMaxNodes]>(Ps + 1024);
   const int64_t new0 = (int64_t)b * p.n;
-  const int row = rb * 128 + tid;
-  const bool valid = tid < 128 && row < R;
+  const int row = rb * kRows + tid;
+  const bool valid = tid < kRows && row < R;
   const int64_t out = valid ? (new0 + row / G) * p.h_q + h * G + row % G : 0;
-  if (tid < 128) load_row_to_tile<D>(Qs, tid, static_cast<const bf16*>(p.q) + out * D, valid);
+  if (tid < kRows) load_row_to_tile<D>(Qs + (tid >> 7) * QB, tid & 127, static_cast<const bf16*>(p.q) + out * D, valid);
   const bf16* kn = static_cast<const bf16*>(p.k_new) + (new0 * p.h_kv + h) * D;
   const bf16* vn = static_cast<const bf16*>(p.v_new) + (new0 * p.h_kv + h) * D;
   const int64_t nrs = (int64_t)p.h_kv * D;
   tree_ancestors(p.parents + new0, p.n, par, anc, tid);
   if (t0 == 0 && nit > 0) {
-    for (int x = tid; x < 64 * (D / 8); x += kTtThreads) {
+    for (int x = tid; x < 64 * (D / 8); x += kThreads) {
       const int r = x / (D / 8), c = x % (D / 8);
       uint4 kx = make_uint4(0u, 0u, 0u, 0u), vx = kx;
       if (r < p.n) {
@@ -162,7 +170,7 @@ __global__ void __launch_bounds__(kTtThreads, 2) tree_attn_tc_kernel(const __gri
   if (tid < p.n && anc[0][tid] != 0ull) atomicMax(&lo_max_s, tree_low(p, len + __popcll(anc[0][tid]) - 1));
   __syncthreads();
   if (t0 == 0 && nit > 0 && bad_s[0] != 0ull)
-    for (int x = tid; x < 64 * (D / 8); x += kTtThreads)
+    for (int x = tid; x < 64 * (D / 8); x += kThreads)
       if (bad_s[0] >> (x / (D / 8)) & 1ull) *reinterpret_cast<uint4*>(tile_at(Vs, x / (D / 8), x % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
   fence_async_smem();
   tc_fence_before();
@@ -171,10 +179,10 @@ __global__ void __launch_bounds__(kTtThreads, 2) tree_attn_tc_kernel(const __gri
   const int lo_max = lo_max_s;
   if (abort_s) nit = 0;
   __syncthreads();                                         // nobody has set it on the way
-  const uint32_t tmem = tmem_base_s, tS = tmem, tO = tmem + 128;
+  const uint32_t tmem = tmem_base_s, tS = tmem, tO = tmem + 128 * TG;       // S: 2 buffers of 64 columns a group, O: D columns a group
 
   const float sl2 = p.scale * kLog2E;
-  if (warp == 5) {
+  if (warp == kLoadWarp) {
     // ---- producer: K of a tile one step before its V, the order in which their places become free ---------------------
     const int first = c0 + max(t0, 1) - 1;                 // chunk of this CTA's first page tile
     int ids = 0, pg = 0, k_issued = 0, v_issued = 0;
@@ -227,63 +235,86 @@ __global__ void __launch_bounds__(kTtThreads, 2) tree_attn_tc_kernel(const __gri
       for (int it = max(0, k_issued - NS); it < k_issued; ++it) wait_for(&k_full[it % NS], (it / NS) & 1);   // no copy outlives the CTA
       for (int it = max(0, v_issued - NS); it < v_issued; ++it) wait_for(&v_full[it % NS], (it / NS) & 1);
     }
-  } else if (warp == 4) {
+  } else if (warp == kMmaWarp) {
     // ---- products -----------------------------------------------------------------------------------------------------
-    if (lane == 0 && nit > 0) {
+    // The whole warp runs the loop and one elected lane issues: descriptors then live in uniform registers, where the
+    // instruction takes them from (issued from a lane's own branch, each of them is moved there first).
+    if (nit > 0) {
       constexpr uint32_t idesc_qk = idesc_bf16(128, 64, 0);
       constexpr uint32_t idesc_pv = idesc_bf16(128, D, 1);
-      const DescWords q_d = desc_words_sw128(smem_u32(Qs), 16, 1024), k_d = desc_words_sw128(smem_u32(Ks), 16, 1024),
-                      p_d = desc_words_sw128(smem_u32(Ps), 16, 1024), v_d = desc_words_sw128(smem_u32(Vs), 8192, 1024);
+      const uint64_t q_d = desc_sw128(smem_u32(Qs), 16, 1024), k_d = desc_sw128(smem_u32(Ks), 16, 1024),
+                     p_d = desc_sw128(smem_u32(Ps), 16, 1024), v_d = desc_sw128(smem_u32(Vs), 8192, 1024);
       auto issue_qk = [&](int it) {
-        const uint32_t kb = k_d.lo + (it % NS) * (TB >> 4), ts = tS + (it & 1) * 64;
-        mma_ss_w<false>(ts, q_d.lo, q_d.hi, kb, k_d.hi, idesc_qk);
+        if (elect_one()) {
+          const uint64_t kb = k_d + (it % NS) * (TB >> 4);
 #pragma unroll
-        for (int kk = 1; kk < D / 16; ++kk)
-          mma_ss_w<true>(ts, q_d.lo + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), q_d.hi, kb + (((kk >> 2) * 8192 + (kk & 3) * 32) >> 4),
-                         k_d.hi, idesc_qk);
-        mma_commit(&s_full[it & 1]);
-        mma_commit(&k_free[it % NS]);
+          for (int g = 0; g < TG; ++g) {
+            const uint64_t qa = q_d + g * (QB >> 4);
+            const uint32_t ts = tS + g * 128 + (it & 1) * 64;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+              mma_ss(ts, qa + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), kb + (((kk >> 2) * 8192 + (kk & 3) * 32) >> 4), idesc_qk, kk > 0);
+            mma_commit(&s_full[2 * g + (it & 1)]);
+          }
+          mma_commit(&k_free[it % NS]);
+        }
+        __syncwarp();
       };
       bool ok = wait_for(&k_full[0], 0);
+      ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
         issue_qk(0);
       }
       for (int it = 0; ok && it < nit; ++it) {
-        if (abort_s) break;
-        if (it + 1 < nit) {                                // its S buffer was consumed before the arrivals on p_full of it - 1
-          ok = wait_for(&k_full[(it + 1) % NS], ((it + 1) / NS) & 1);
+        if (__any_sync(0xffffffffu, abort_s)) break;
+        if (it + 1 < nit) {                                // its S buffers were consumed before the arrivals on p_full of it - 1
+          ok = __all_sync(0xffffffffu, wait_for(&k_full[(it + 1) % NS], ((it + 1) / NS) & 1));
           if (!ok) break;
           tc_fence_after();
           issue_qk(it + 1);
         }
-        ok = wait_for(p_full, it & 1) && wait_for(&v_full[it % NS], (it / NS) & 1);
+        ok = __all_sync(0xffffffffu, wait_for(&v_full[it % NS], (it / NS) & 1));
         if (!ok) break;
-        tc_fence_after();
-        const uint32_t b0 = v_d.lo + (it % NS) * (TB >> 4);
-        mma_ss_wr(tO, p_d.lo, p_d.hi, b0, v_d.hi, idesc_pv, it > 0 ? 1u : 0u);
+        const uint64_t b0 = v_d + (it % NS) * (TB >> 4);
 #pragma unroll
-        for (int kk = 1; kk < 4; ++kk) mma_ss_w<true>(tO, p_d.lo + ((kk * 32) >> 4), p_d.hi, b0 + ((kk * 2048) >> 4), v_d.hi, idesc_pv);
-        mma_commit(&v_free[it % NS]);
+        for (int g = 0; g < TG; ++g) {
+          ok = ok && __all_sync(0xffffffffu, wait_for(&p_full[g], it & 1));
+          if (ok) {
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t pa = p_d + g * (16384 >> 4);
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_ss(tO + g * D, pa + ((kk * 32) >> 4), b0 + ((kk * 2048) >> 4), idesc_pv, it > 0 || kk > 0);
+              mma_commit(&pv_done[g]);
+              if (g == TG - 1) mma_commit(&v_free[it % NS]);
+            }
+            __syncwarp();
+          }
+        }
+        if (!ok) break;
       }
-      if (!ok) { abort_s = 1; atomicExch(&g_tree_tc_expired, 8300002); }
-      mma_commit(done);                                    // no product outlives the CTA's tensor memory
+      if (!ok && lane == 0) { abort_s = 1; atomicExch(&g_tree_tc_expired, 8300002); }
+      if (elect_one()) mma_commit(done);                   // no product outlives the CTA's tensor memory
       wait_for(done, 0);
     }
   } else {
     // ---- rows -----------------------------------------------------------------------------------------------------------
-    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-    const bool rows_here = rb * 128 + warp * 32 < R;
+    const int grp = tid >> 7, r = tid & 127;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, tSg = tS + grp * 128 + lane_base, tOg = tO + grp * D + lane_base;
+    uint8_t* Pg = Ps + grp * 16384;
+    const bool rows_here = rb * kRows + warp * 32 < R;
     float m = -CUDART_INF_F, l = 0.f;                      // reference point (log2 units) and sum
     bool ok = true;
     for (int it = 0; it < nit; ++it) {
       const int s = it & 1, t = t0 + it, c = c0 + t - 1, vs = it % NS;
-      ok = wait_for(&s_full[s], (it >> 1) & 1);
+      ok = wait_for(&s_full[2 * grp + s], (it >> 1) & 1);
       tc_fence_after();
       float sv[64];
       if (rows_here) {
-        tmem_ld32(tS + lane_base + s * 64, sv);
-        tmem_ld32(tS + lane_base + s * 64 + 32, sv + 32);
+        tmem_ld32(tSg + s * 64, sv);
+        tmem_ld32(tSg + s * 64 + 32, sv + 32);
       }
       // (k_full of this tile cannot be asked here: with the product done the next tile of the place may have arrived too)
       const bool in_pool = tile_ok[it & 7] != 0;
@@ -322,7 +353,7 @@ __global__ void __launch_bounds__(kTtThreads, 2) tree_attn_tc_kernel(const __gri
         }
         l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
       }
-      if (it > 0) ok = wait_for(&v_free[(it - 1) % NS], ((it - 1) / NS) & 1) && ok;     // P is free, O stands still
+      if (it > 0) ok = wait_for(&pv_done[grp], (it - 1) & 1) && ok;     // P is free, O stands still
       ok = __all_sync(0xffffffffu, ok) && !abort_s;
       if (!ok) break;
       if (rows_here) {
@@ -332,47 +363,51 @@ __global__ void __launch_bounds__(kTtThreads, 2) tree_attn_tc_kernel(const __gri
 #pragma unroll 1
           for (int cb = 0; cb < D / 32; ++cb) {
             float ov[32];
-            tmem_ld32(tO + lane_base + cb * 32, ov);
+            tmem_ld32(tOg + cb * 32, ov);
             tmem_ld_wait32(ov);
 #pragma unroll
             for (int j = 0; j < 32; ++j) ov[j] *= f;
-            tmem_st32(tO + lane_base + cb * 32, ov);
+            tmem_st32(tOg + cb * 32, ov);
           }
           tmem_st_wait();
         }
-        store_row_bf16_sw128(Ps, tid, sv);
+        store_row_bf16_sw128(Pg, r, sv);
       }
-      // V rows of this page that nobody sees become zeros, and so do those that some rows see and that are not finite
-      if (t > 0 && tid < 64) {
+      // V rows of this page that nobody sees become zeros (one warp, a row at a time), and so do those that some rows see
+      // and others do not and that are not finite
+      if (t > 0 && warp < 2) {
         const u64t held = in_pool ? tree_page_mask(p, c, len, lo_min) : 0ull;
-        const bool mixed = lo_max > c * 64 && c - c0 < 2;
-        bool clear = !(held >> tid & 1ull);
-        if (clear || mixed) {
+        uint8_t* tile = Vs + vs * TB;
+        if (warp == 0 && held != ~0ull) {
           ok = wait_for(&v_full[vs], (it / NS) & 1);
-          uint8_t* tile = Vs + vs * TB;
-          if (!clear) {
+          for (u64t rest = ~held; rest; rest &= rest - 1)
+            if (lane < D / 8) *reinterpret_cast<uint4*>(tile_at(tile, __ffsll((long long)rest) - 1, lane)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (lo_max > c * 64 && c - c0 < 2 && (held >> tid & 1ull)) {
+          ok = wait_for(&v_full[vs], (it / NS) & 1) && ok;
+          bool clear = false;
 #pragma unroll
-            for (int e = 0; e < D / 8; ++e) clear = clear || not_finite8(*reinterpret_cast<const uint4*>(tile_at(tile, tid, e)));
-            if (clear) atomicOr(&bad_s[1 + c - c0], 1ull << tid);
-          }
-          if (clear)
+          for (int e = 0; e < D / 8; ++e) clear = clear || not_finite8(*reinterpret_cast<const uint4*>(tile_at(tile, tid, e)));
+          if (clear) {
+            atomicOr(&bad_s[1 + c - c0], 1ull << tid);
 #pragma unroll
             for (int e = 0; e < D / 8; ++e) *reinterpret_cast<uint4*>(tile_at(tile, tid, e)) = make_uint4(0u, 0u, 0u, 0u);
+          }
         }
       }
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_async_smem();
       tc_fence_before();
-      mbar_arrive(p_full);
+      mbar_arrive(&p_full[grp]);
     }
-    if (ok && nit > 0) ok = __all_sync(0xffffffffu, wait_for(&v_free[(nit - 1) % NS], ((nit - 1) / NS) & 1)) && !abort_s;
+    if (ok && nit > 0) ok = __all_sync(0xffffffffu, wait_for(&pv_done[grp], (nit - 1) & 1)) && !abort_s;
     if (!ok && lane == 0) {
       abort_s = 1;
       atomicExch(&g_tree_tc_expired, 8300003);
     }
     if (ok) tc_fence_after();
-    named_bar_sync(1, 128);                                // bad_s of all row threads
+    named_bar_sync(1, kRows);                              // bad_s of all row threads
     const bool have = ok && nit > 0 && rows_here;
     const float inv = p.splits > 1 ? 1.f : (l > 0.f ? 1.f / l : (l == l ? 0.f : l));
     const int64_t at = (int64_t)split * p.B * p.n * p.h_q + out;
@@ -380,7 +415,7 @@ __global__ void __launch_bounds__(kTtThreads, 2) tree_attn_tc_kernel(const __gri
     for (int cb = 0; cb < D / 32; ++cb) {
       float ov[32];
       if (have) {
-        tmem_ld32(tO + lane_base + cb * 32, ov);
+        tmem_ld32(tOg + cb * 32, ov);
         tmem_ld_wait32(ov);
       } else {
 #pragma unroll
@@ -412,7 +447,7 @@ __global__ void __launch_bounds__(kTtThreads, 2) tree_attn_tc_kernel(const __gri
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) tmem_dealloc(tmem, 256);
+  if (warp == kMmaWarp) tmem_dealloc(tmem, kTmem);
 }
 
 int take_status_tree_tc() {
@@ -425,20 +460,23 @@ int take_status_tree_tc() {
   return x != 0 ? x : v;
 }
 
-template <int D>
+template <int D, int TG>
 static int launch_tree_tc(const TreeParams& p, cudaStream_t st) {
   CUtensorMap tmK, tmV;
   const uint64_t rows = (uint64_t)p.num_pages * p.h_kv * 64;
   if (int rc = make_tmap_bf16_rows(&tmK, p.k_pages, rows, D, D, 64)) return rc;
   if (int rc = make_tmap_bf16_rows(&tmV, p.v_pages, rows, D, D, 64)) return rc;
-  cudaFuncSetAttribute(tree_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, TtShape<D>::SMEM);
-  tree_attn_tc_kernel<D><<<dim3((unsigned)(p.row_blocks * p.splits), (unsigned)p.h_kv, (unsigned)p.B), kTtThreads, TtShape<D>::SMEM, st>>>(p, tmK, tmV);
+  using Sh = TtShape<D, TG>;
+  cudaFuncSetAttribute(tree_attn_tc_kernel<D, TG>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
+  tree_attn_tc_kernel<D, TG><<<dim3((unsigned)(p.row_blocks * p.splits), (unsigned)p.h_kv, (unsigned)p.B), Sh::THREADS, Sh::SMEM, st>>>(p, tmK, tmV);
   HILS_LAUNCH_CHECK("tree_attn_paged (tensor-core path)");
   return HILS_OK;
 }
 
-int tree_tc_launch(const TreeParams& p, int D, cudaStream_t st) {
-  return D == 128 ? launch_tree_tc<128>(p, st) : launch_tree_tc<64>(p, st);
+// rows_per_cta: 128 or 256
+int tree_tc_launch(const TreeParams& p, int D, int rows_per_cta, cudaStream_t st) {
+  if (rows_per_cta == 256) return D == 128 ? launch_tree_tc<128, 2>(p, st) : launch_tree_tc<64, 2>(p, st);
+  return D == 128 ? launch_tree_tc<128, 1>(p, st) : launch_tree_tc<64, 1>(p, st);
 }
 
 }  // namespace hils

@@ -121,6 +121,12 @@ __device__ __forceinline__ void mma_ss_wr(uint32_t tmem_d, uint32_t a_lo, uint32
       ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// one lane of a converged warp; the compiler keeps what surrounds it in uniform registers, which the MMA wants
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(ok));
+  return ok != 0;
+}
 // arrive on `bar` when all MMAs issued so far by this thread have completed
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
