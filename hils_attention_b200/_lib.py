@@ -94,6 +94,7 @@ _lib: Optional[C.CDLL] = None
 
 class HilsError(RuntimeError):
     """Raised when a C-ABI call returns a non-zero status."""
+    status = 0
 
 
 def load() -> C.CDLL:
@@ -140,11 +141,11 @@ def _call_device() -> Optional[torch.device]:
     if not devs:
         return None
     first = devs[0]
-    for d in devs[1:]:
-        if d != first:
-            devs.clear()
-            raise RuntimeError(f"hils_b200: tensors of one call live on different devices ({first} and {d}); "
-                               "nothing was launched")
+    if devs.count(first) != len(devs):
+        d = next(d for d in devs if d != first)
+        devs.clear()
+        raise RuntimeError(f"hils_b200: tensors of one call live on different devices ({first} and {d}); "
+                           "nothing was launched")
     return first
 
 
@@ -177,6 +178,21 @@ def stream() -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)       # the same handle without building a Stream object per call
 
 
+ERR_WORKSPACE = -4
+
+
+def call_or_workspace(name: str, *args) -> bool:
+    """`call`, but False instead of an error when the workspace given is too small (nothing was launched then): a caller that
+    hands the same workspace in again and again need not ask for its size every time."""
+    try:
+        call(name, *args)
+        return True
+    except HilsError as e:
+        if e.status != ERR_WORKSPACE:
+            raise
+        return False
+
+
 def call(name: str, *args):
     """Invoke a status-returning entry point and raise HilsError on failure.  The call runs with the
     tensors' device current (tensor maps, symbol addresses and launches bind to the current context)."""
@@ -192,7 +208,9 @@ def call(name: str, *args):
     _launches += KERNELS_PER_CALL.get(name, 1)
     if rc != 0:
         msg = lib.hils_last_error().decode("utf-8", "replace")
-        raise HilsError(f"{name} failed with status {rc}: {msg}")
+        err = HilsError(f"{name} failed with status {rc}: {msg}")
+        err.status = rc
+        raise err
     if _CHECK_STATUS:
         st = int(lib.hils_take_device_status())
         if st != 0:

@@ -33,6 +33,7 @@ int take_status_paged();
 int take_status_pages();
 int take_status_tree();
 int take_status_tree_tc();
+int take_status_tree_mma();
 }  // namespace hils
 
 extern "C" int hils_version(void) { return 100; }
@@ -49,9 +50,10 @@ extern "C" int hils_take_device_status(void) {
   const int g = hils::take_status_pages();
   const int h = hils::take_status_tree();
   const int i = hils::take_status_tree_tc();
-  for (const int v : {a, b, c, d, e, f, g, h, i})
+  const int j = hils::take_status_tree_mma();
+  for (const int v : {a, b, c, d, e, f, g, h, i, j})
     if (v < 0) return -1;
-  for (const int v : {a, b, c, d, e, f, g, h, i})
+  for (const int v : {a, b, c, d, e, f, g, h, i, j})
     if (v != 0) return v;
   return 0;
 }

@@ -5,6 +5,9 @@
 #include <algorithm>
 
 #include "tree_common.cuh"
+#ifndef TREE_MMA_ROWS
+#define TREE_MMA_ROWS 32
+#endif
 
 namespace hils {
 
@@ -34,7 +37,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeParams p) {
   bool over;
   const int len = tree_length(p, b, over);
   if (over && tid == 0) atomicExch(&g_tree_status, 8200002);
-  tree_ancestors(p.parents + (int64_t)b * p.n, p.n, par_s, anc_s, tid);
+  tree_ancestors(tree_parent(p.parents + (int64_t)b * p.n, p.n, tid), par_s, anc_s, tid, 0, kTreeThreads);
   const u64t* anc = anc_s[0];
   if (tid < kTreeRows) {
     const int row = rb * kTreeRows + tid, j = row / G;
@@ -228,7 +231,7 @@ __global__ void __launch_bounds__(kTreeMaxNodes) tree_positions_kernel(const int
   __shared__ int par_s[2][kTreeMaxNodes];
   __shared__ u64t anc_s[2][kTreeMaxNodes];
   const int b = blockIdx.x, j = threadIdx.x;
-  tree_ancestors(parents + (int64_t)b * n, n, par_s, anc_s, j);
+  tree_ancestors(tree_parent(parents + (int64_t)b * n, n, j), par_s, anc_s, j, 0, kTreeMaxNodes);
   if (j < n) pos[(int64_t)b * n + j] = anc_s[0][j] ? max(lens[b], 0) + __popcll(anc_s[0][j]) - 1 : -1;
 }
 
@@ -250,8 +253,12 @@ static int tree_splits(int64_t ctas, int tiles, int slots) {
   return best;
 }
 
-// rows of one key head that a CTA takes
-static int tree_cta_rows(int64_t R, int dtype) { return dtype != HILS_BF16 ? kTreeRows : (R > 128 ? 256 : 128); }
+// Rows of one key head that a CTA takes.  fp32: the CUDA-core kernel's tile.  bf16: up to 32 rows the warp-level kernel
+// (tree_attn_mma.cu), up to 128 and above the tcgen05 kernels with one and two row groups (tree_attn_tc.cu).
+static int tree_cta_rows(int64_t R, int dtype) {
+  if (dtype != HILS_BF16) return kTreeRows;
+  return R <= TREE_MMA_ROWS ? (R <= 16 ? 16 : 32) : (R <= 128 ? 128 : 256);
+}
 
 static TreeParams tree_plan(int B, int n, int h_q, int h_kv, int max_len, int W, int dtype) {
   TreeParams p = {};
@@ -276,11 +283,13 @@ int take_status_tree() {
 }
 
 int tree_tc_launch(const TreeParams& p, int D, int rows_per_cta, cudaStream_t st);   // tree_attn_tc.cu
+int tree_mma_launch(const TreeParams& p, int D, int rows, cudaStream_t st);           // tree_attn_mma.cu
 
 template <typename T, int D>
 static int launch_tree(const TreeParams& p, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
-    if (int rc = tree_tc_launch(p, D, tree_cta_rows((int64_t)p.n * (p.h_q / p.h_kv), HILS_BF16), st)) return rc;
+    const int rows = tree_cta_rows((int64_t)p.n * (p.h_q / p.h_kv), HILS_BF16);
+    if (int rc = rows <= 32 ? tree_mma_launch(p, D, rows, st) : tree_tc_launch(p, D, rows, st)) return rc;
   } else {
     const size_t smem = tree_smem_floats<D>() * sizeof(float);
     cudaFuncSetAttribute(tree_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

@@ -108,7 +108,10 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
   }
   const int G = p.h_q / p.h_kv, R = p.n * G;
   const int rb = blockIdx.x % p.row_blocks, split = blockIdx.x / p.row_blocks, h = blockIdx.y, b = blockIdx.z;
-  if (tid == 0) {
+  bool over;
+  const int len = tree_length(p, b, over);
+  const int parent = tree_parent(p.parents + (int64_t)b * p.n, p.n, tid);
+  if (tid == 32 * kLoadWarp) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_free[s], 1);
@@ -126,60 +129,68 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
     abort_s = *const_cast<volatile int*>(&g_tree_tc_expired) != 0;
     lo_max_s = 0;
     bad_s[0] = bad_s[1] = bad_s[2] = 0ull;
+    if (over) atomicExch(&g_tree_tc_status, 8200002);
   }
   if (warp == kMmaWarp) tmem_alloc(&tmem_base_s, kTmem);
-  bool over;
-  const int len = tree_length(p, b, over);
-  if (over && tid == 0) atomicExch(&g_tree_tc_status, 8200002);
   const int lo_min = tree_low(p, len), c0 = lo_min >> 6, c1 = (len + 63) >> 6;
   const int nt = 1 + max(0, c1 - c0), per = (nt + p.splits - 1) / p.splits;
   const int t0 = split * per;
-  int nit = max(0, min(nt, t0 + per) - t0);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s, tS = tmem, tO = tmem + 128 * TG;       // S: 2 buffers of 64 columns a group, O: D columns a group
+  const int nit = abort_s ? 0 : max(0, min(nt, t0 + per) - t0);
+  __syncthreads();                                         // nobody has set abort_s on the way
 
-  // ---- ancestors, rows, drafted keys (the scratch lies where P will be) --------------------------------------------
-  int (*par)[kTreeMaxNodes] = reinterpret_cast<int (*)[kTreeMaxNodes]>(Ps);
-  u64t (*anc)[kTreeMaxNodes] = reinterpret_cast<u64t (*)[kTreeMaxNodes]>(Ps + 1024);
+  // ---- ancestors, rows, drafted keys (the scratch lies where P will be); the producer is already on its way ------------
   const int64_t new0 = (int64_t)b * p.n;
   const int row = rb * kRows + tid;
   const bool valid = tid < kRows && row < R;
   const int64_t out = valid ? (new0 + row / G) * p.h_q + h * G + row % G : 0;
-  if (tid < kRows) load_row_to_tile<D>(Qs + (tid >> 7) * QB, tid & 127, static_cast<const bf16*>(p.q) + out * D, valid);
   const bf16* kn = static_cast<const bf16*>(p.k_new) + (new0 * p.h_kv + h) * D;
   const bf16* vn = static_cast<const bf16*>(p.v_new) + (new0 * p.h_kv + h) * D;
   const int64_t nrs = (int64_t)p.h_kv * D;
-  tree_ancestors(p.parents + new0, p.n, par, anc, tid);
-  if (t0 == 0 && nit > 0) {
-    for (int x = tid; x < 64 * (D / 8); x += kThreads) {
-      const int r = x / (D / 8), c = x % (D / 8);
-      uint4 kx = make_uint4(0u, 0u, 0u, 0u), vx = kx;
-      if (r < p.n) {
-        kx = *reinterpret_cast<const uint4*>(kn + r * nrs + c * 8);
-        vx = *reinterpret_cast<const uint4*>(vn + r * nrs + c * 8);
-        if (not_finite8(vx)) atomicOr(&bad_s[0], 1ull << r);
+  int lo = 0x7fffffff, lo_max = 0;
+  u64t dmask = 0ull;
+  if (warp != kLoadWarp) {
+    constexpr int kMeet = kThreads - 32;
+    int (*par)[kTreeMaxNodes] = reinterpret_cast<int (*)[kTreeMaxNodes]>(Ps);
+    u64t (*anc)[kTreeMaxNodes] = reinterpret_cast<u64t (*)[kTreeMaxNodes]>(Ps + 1024);
+    if (t0 == 0 && nit > 0) {
+      for (int x = tid; x < 64 * (D / 8); x += kMeet) {
+        const int r = x / (D / 8), c = x % (D / 8);
+        uint4 kx = make_uint4(0u, 0u, 0u, 0u), vx = kx;
+        if (r < p.n) {
+          kx = *reinterpret_cast<const uint4*>(kn + r * nrs + c * 8);
+          vx = *reinterpret_cast<const uint4*>(vn + r * nrs + c * 8);
+          if (not_finite8(vx)) {                           // zero in the product, added row by row at the end
+            atomicOr(&bad_s[0], 1ull << r);
+            vx = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        *reinterpret_cast<uint4*>(tile_at(Ks, r, c)) = kx;
+        *reinterpret_cast<uint4*>(tile_at(Vs, r, c)) = vx;
       }
-      *reinterpret_cast<uint4*>(tile_at(Ks, r, c)) = kx;
-      *reinterpret_cast<uint4*>(tile_at(Vs, r, c)) = vx;
+    }
+    if (tid < kRows) load_row_to_tile<D>(Qs + (tid >> 7) * QB, tid & 127, static_cast<const bf16*>(p.q) + out * D, valid);
+    tree_ancestors(parent, par, anc, tid, 2, kMeet);
+    if (valid && anc[0][row / G] != 0ull) {
+      lo = tree_low(p, len + __popcll(anc[0][row / G]) - 1);
+      dmask = tree_draft_mask(p, anc[0], row / G, len, lo);
+    }
+    if (tid < p.n && anc[0][tid] != 0ull) atomicMax(&lo_max_s, tree_low(p, len + __popcll(anc[0][tid]) - 1));
+    named_bar_sync(2, kMeet);
+    if (t0 == 0 && nit > 0 && bad_s[0] != 0ull)            // the other pieces of those rows
+      for (int x = tid; x < 64 * (D / 8); x += kMeet)
+        if (bad_s[0] >> (x / (D / 8)) & 1ull) *reinterpret_cast<uint4*>(tile_at(Vs, x / (D / 8), x % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
+    fence_async_smem();
+    named_bar_sync(2, kMeet);
+    lo_max = lo_max_s;
+    if (t0 == 0 && nit > 0 && tid == 0) {                  // the drafted tile is there
+      mbar_arrive(&k_full[0]);
+      mbar_arrive(&v_full[0]);
     }
   }
-  int lo = 0x7fffffff;
-  u64t dmask = 0ull;
-  if (valid && anc[0][row / G] != 0ull) {
-    lo = tree_low(p, len + __popcll(anc[0][row / G]) - 1);
-    dmask = tree_draft_mask(p, anc[0], row / G, len, lo);
-  }
-  if (tid < p.n && anc[0][tid] != 0ull) atomicMax(&lo_max_s, tree_low(p, len + __popcll(anc[0][tid]) - 1));
-  __syncthreads();
-  if (t0 == 0 && nit > 0 && bad_s[0] != 0ull)
-    for (int x = tid; x < 64 * (D / 8); x += kThreads)
-      if (bad_s[0] >> (x / (D / 8)) & 1ull) *reinterpret_cast<uint4*>(tile_at(Vs, x / (D / 8), x % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
-  fence_async_smem();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const int lo_max = lo_max_s;
-  if (abort_s) nit = 0;
-  __syncthreads();                                         // nobody has set it on the way
-  const uint32_t tmem = tmem_base_s, tS = tmem, tO = tmem + 128 * TG;       // S: 2 buffers of 64 columns a group, O: D columns a group
 
   const float sl2 = p.scale * kLog2E;
   if (warp == kLoadWarp) {
@@ -187,8 +198,9 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
     const int first = c0 + max(t0, 1) - 1;                 // chunk of this CTA's first page tile
     int ids = 0, pg = 0, k_issued = 0, v_issued = 0;
     bool ok = true;
-    auto bring = [&](uint64_t* full, uint8_t* tile, const CUtensorMap* map, bool load, int page) {
-      if (!load) {
+    auto bring = [&](uint64_t* full, uint8_t* tile, const CUtensorMap* map, bool draft, int page) {
+      if (draft) return;                                   // written and announced by the other warps
+      if ((unsigned)page >= (unsigned)p.num_pages) {
         mbar_arrive(full);
         return;
       }
@@ -214,7 +226,7 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
             const bool in_pool = (unsigned)pg < (unsigned)p.num_pages;
             tile_ok[step & 7] = in_pool;                   // reaches the row threads through k_full and s_full; they are past step - 8
             if (!in_pool) atomicExch(&g_tree_tc_status, 8200001);
-            bring(&k_full[s], Ks + s * TB, &tmK, t0 + step > 0 && in_pool, pg);
+            bring(&k_full[s], Ks + s * TB, &tmK, t0 + step == 0, pg);
             ++k_issued;
           }
         }
@@ -222,7 +234,7 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
           const int it = step - 1, s = it % NS;
           if (it >= NS) ok = wait_for(&v_free[s], (it / NS - 1) & 1);
           if (ok) {
-            bring(&v_full[s], Vs + s * TB, &tmV, t0 + it > 0 && (unsigned)prev < (unsigned)p.num_pages, prev);
+            bring(&v_full[s], Vs + s * TB, &tmV, t0 + it == 0, prev);
             ++v_issued;
           }
         }

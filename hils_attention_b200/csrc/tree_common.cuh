@@ -29,14 +29,17 @@ struct TreeParams {
 
 // Ancestors of the tree's nodes.  anc[j]: bits of j and its ancestors, 0 when j is absent: its parent is no earlier node
 // and not -1, or an ancestor is absent.  Pointer doubling: six rounds cover 64 nodes, and a bad parent cannot make it loop.
-// Called by all threads of a CTA of at least 64; par and anc: [2][64] in shared memory; the result is in anc[0].
-__device__ __forceinline__ void tree_ancestors(const int32_t* parents, int n, int (*par)[kTreeMaxNodes], u64t (*anc)[kTreeMaxNodes], int tid) {
+// Called by `threads` threads (at least 64, thread 0 among them) that meet at barrier `bar`; parent: that of node tid, which
+// the caller loads early; par and anc: [2][64] in shared memory; the result is in anc[0].
+__device__ __forceinline__ int tree_parent(const int32_t* parents, int n, int tid) { return tid < min(n, kTreeMaxNodes) ? parents[tid] : -2; }
+
+__device__ __forceinline__ void tree_ancestors(int parent, int (*par)[kTreeMaxNodes], u64t (*anc)[kTreeMaxNodes], int tid, int bar, int threads) {
+  auto meet = [&] { asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads) : "memory"); };
   if (tid < kTreeMaxNodes) {
-    const int pj = tid < n ? parents[tid] : -2;
-    par[0][tid] = (pj >= -1 && pj < tid) ? pj : -2;      // -2: absent
+    par[0][tid] = (parent >= -1 && parent < tid) ? parent : -2;      // -2: absent
     anc[0][tid] = 1ull << tid;
   }
-  __syncthreads();
+  meet();
 #pragma unroll
   for (int r = 0; r < 6; ++r) {
     const int a = r & 1;
@@ -45,10 +48,10 @@ __device__ __forceinline__ void tree_ancestors(const int32_t* parents, int n, in
       par[a ^ 1][tid] = pj >= 0 ? par[a][pj] : pj;
       anc[a ^ 1][tid] = pj >= 0 ? (anc[a][tid] | anc[a][pj]) : anc[a][tid];
     }
-    __syncthreads();
+    meet();
   }
   if (tid < kTreeMaxNodes && par[0][tid] != -1) anc[0][tid] = 0ull;
-  __syncthreads();
+  meet();
 }
 
 __device__ __forceinline__ int tree_low(const TreeParams& p, int t) {      // leftmost position visible from position t

@@ -22,7 +22,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import F32, call, dtype_code, ptr, query, stream
+from ._lib import F32, call, call_or_workspace, dtype_code, ptr, query, stream
 
 __all__ = [
     "chunk_attn_pool", "chunk_attn_pool_tilelang", "chunk_mean_pool", "online_softmax_topk_head",
@@ -535,37 +535,45 @@ def tree_attn_paged(q, k_new, v_new, k_pages, v_pages, page_table, lens, max_len
     when expand_to_chunk), landmark positions excepted when mask_lmk, as flex_attn_tl.  The pages are only read: the
     accepted tokens are written by commit_drafts.
     Returns o (B, n, h_q, D), lse (B, n, h_q) fp32 (0 and -inf for rows that see nothing) and the workspace for reuse."""
-    if q.dim() != 4 or k_new.dim() != 4 or k_new.shape != v_new.shape or k_new.shape[:2] != q.shape[:2] or k_new.shape[3] != q.shape[3]:
-        raise ValueError(f"tree_attn_paged: q (B,n,h_q,D), k_new and v_new (B,n,h_kv,D), got {tuple(q.shape)}, {tuple(k_new.shape)}, "
-                         f"{tuple(v_new.shape)}")
-    B, n, h_q, D = q.shape
-    h_kv = k_new.shape[2]
-    if k_pages.shape != v_pages.shape or k_pages.dim() != 4 or k_pages.shape[1:] != (h_kv, chunk_size, D):
+    if q.dim() != 4 or k_new.dim() != 4:
+        raise ValueError(f"tree_attn_paged: q (B,n,h_q,D), k_new and v_new (B,n,h_kv,D), got {tuple(q.shape)}, {tuple(k_new.shape)}")
+    (B, n, h_q, D), h_kv, dtype = q.shape, k_new.shape[2], q.dtype
+    if k_new.shape != (B, n, h_kv, D) or v_new.shape != (B, n, h_kv, D):
+        raise ValueError(f"tree_attn_paged: q {tuple(q.shape)} with k_new {tuple(k_new.shape)}, v_new {tuple(v_new.shape)}")
+    pages = k_pages.shape[0]
+    if k_pages.shape != (pages, h_kv, chunk_size, D) or v_pages.shape != (pages, h_kv, chunk_size, D):
         raise ValueError(f"tree_attn_paged: pools {tuple(k_pages.shape)} / {tuple(v_pages.shape)} for {h_kv} heads of {D} in pages of {chunk_size}")
     if page_table.dim() != 2 or page_table.shape[0] != B or lens.shape != (B,) or parents.shape != (B, n):
         raise ValueError(f"tree_attn_paged: page_table {tuple(page_table.shape)}, lens {tuple(lens.shape)}, parents {tuple(parents.shape)} "
                          f"for {B} sequences of {n} nodes")
-    if page_table.dtype != torch.int32 or lens.dtype != torch.int32 or parents.dtype != torch.int32:
+    i32 = torch.int32
+    if page_table.dtype != i32 or lens.dtype != i32 or parents.dtype != i32:
         raise TypeError("tree_attn_paged: page_table, lens and parents must be int32")
     dt = dtype_code(q)
-    for t in (k_new, v_new, k_pages, v_pages):
-        if t.dtype != q.dtype:
-            raise TypeError(f"tree_attn_paged: q of {q.dtype}, keys or values of {t.dtype}")
-    for t in (q, k_new, v_new, k_pages, v_pages, page_table, lens, parents):
-        if not t.is_contiguous():
-            raise ValueError("tree_attn_paged: tensors must be contiguous")
-    if window_size is not None and window_size < 1:
+    if not (k_new.dtype == v_new.dtype == k_pages.dtype == v_pages.dtype == dtype):
+        raise TypeError(f"tree_attn_paged: q of {dtype}, keys and values of {k_new.dtype}, {v_new.dtype}, {k_pages.dtype}, {v_pages.dtype}")
+    if not (q.is_contiguous() and k_new.is_contiguous() and v_new.is_contiguous() and k_pages.is_contiguous() and v_pages.is_contiguous()
+            and page_table.is_contiguous() and lens.is_contiguous() and parents.is_contiguous()):
+        raise ValueError("tree_attn_paged: tensors must be contiguous")
+    if window_size is None:
+        W = 0
+    elif window_size < 1:
         raise ValueError(f"tree_attn_paged: window_size {window_size} (None for the whole cache)")
-    W = 0 if window_size is None else int(window_size)
-    o = torch.empty_like(q)
-    lse = torch.empty((B, n, h_q), dtype=torch.float32, device=q.device)
-    need = query("hils_tree_attn_paged_workspace_bytes", B, n, h_q, h_kv, D, int(max_len), W, dt)
-    if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    call("hils_tree_attn_paged", ptr(q), ptr(k_new), ptr(v_new), ptr(k_pages), ptr(v_pages), ptr(page_table), page_table.shape[1],
-         k_pages.shape[0], ptr(lens), int(max_len), ptr(parents), ptr(o), ptr(lse), B, n, h_q, h_kv, D, W, int(chunk_size), int(bool(mask_lmk)),
-         int(bool(expand_to_chunk)), 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), dt,
-         ptr(workspace) if workspace.numel() else None, workspace.numel(), stream())
+    else:
+        W = int(window_size)
+    o, lse = torch.empty_like(q), q.new_empty((B, n, h_q), dtype=torch.float32)
+    max_len, asked = int(max_len), workspace is None
+
+    def size():
+        return torch.empty(query("hils_tree_attn_paged_workspace_bytes", B, n, h_q, h_kv, D, max_len, W, dt), dtype=torch.uint8, device=q.device)
+    if asked:
+        workspace = size()
+    args = (ptr(q), ptr(k_new), ptr(v_new), ptr(k_pages), ptr(v_pages), ptr(page_table), page_table.shape[1], pages, ptr(lens), max_len,
+            ptr(parents), ptr(o), ptr(lse), B, n, h_q, h_kv, D, W, chunk_size, 1 if mask_lmk else 0, 1 if expand_to_chunk else 0,
+            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), dt)
+    if not call_or_workspace("hils_tree_attn_paged", *args, ptr(workspace) if workspace.numel() else None, workspace.numel(), stream()):
+        workspace = size()
+        call("hils_tree_attn_paged", *args, ptr(workspace), workspace.numel(), stream())
     return o, lse, workspace
 
 
@@ -680,22 +688,21 @@ def commit_drafts(k_draft, v_draft, k_pages, v_pages, page_table, lens, path) ->
     Node path[b, i] becomes token lens[b] + i; lens is left as it is, no other row is touched."""
     layers, pages, layer_bytes = _pool_layers(k_pages, v_pages, "commit_drafts")
     one = k_pages.dim() == 4
-    if k_draft.shape != v_draft.shape or k_draft.dim() != (4 if one else 5):
+    if k_draft.dim() != (4 if one else 5):
         raise ValueError(f"commit_drafts: drafts {tuple(k_draft.shape)} / {tuple(v_draft.shape)} for pools {tuple(k_pages.shape)}")
-    B, n, h_kv, D = k_draft.shape[-4:]
-    if (not one and k_draft.shape[0] != layers) or k_pages.shape[-3:] != (h_kv, 64, D):
-        raise ValueError(f"commit_drafts: drafts {tuple(k_draft.shape)} do not fit pools {tuple(k_pages.shape)}")
-    if k_draft.dtype != k_pages.dtype or v_draft.dtype != k_pages.dtype:
+    *lead, B, n, h_kv, D = k_draft.shape
+    if v_draft.shape != k_draft.shape or (lead and lead[0] != layers) or k_pages.shape[-3:] != (h_kv, 64, D):
+        raise ValueError(f"commit_drafts: drafts {tuple(k_draft.shape)} / {tuple(v_draft.shape)} do not fit pools {tuple(k_pages.shape)}")
+    if not (k_draft.dtype == v_draft.dtype == k_pages.dtype):
         raise TypeError(f"commit_drafts: drafts of {k_draft.dtype} / {v_draft.dtype}, pools of {k_pages.dtype}")
-    for name, t in (("page_table", page_table), ("lens", lens), ("path", path)):
-        if t.dtype != torch.int32:
-            raise TypeError(f"commit_drafts: {name} must be int32, got {t.dtype}")
+    i32 = torch.int32
+    if page_table.dtype != i32 or lens.dtype != i32 or path.dtype != i32:
+        raise TypeError(f"commit_drafts: page_table, lens and path must be int32, got {page_table.dtype}, {lens.dtype}, {path.dtype}")
     if page_table.dim() != 2 or path.dim() != 2 or page_table.shape[0] != B or lens.shape != (B,) or path.shape[0] != B or path.shape[1] > n:
         raise ValueError(f"commit_drafts: page_table {tuple(page_table.shape)}, lens {tuple(lens.shape)}, path {tuple(path.shape)} for "
                          f"{B} sequences of {n} nodes")
-    for t in (k_draft, v_draft, page_table, lens, path):
-        if not t.is_contiguous():
-            raise ValueError("commit_drafts: drafts, page_table, lens and path must be contiguous")
+    if not (k_draft.is_contiguous() and v_draft.is_contiguous() and page_table.is_contiguous() and lens.is_contiguous() and path.is_contiguous()):
+        raise ValueError("commit_drafts: drafts, page_table, lens and path must be contiguous")
     if B == 0 or layers == 0 or path.shape[1] == 0:
         return
     call("hils_commit_drafts", ptr(k_draft), ptr(v_draft), ptr(k_pages), ptr(v_pages), ptr(page_table), page_table.shape[1], pages, ptr(lens),
@@ -809,49 +816,57 @@ def rope_frequencies(rot: int, base: float = 10000.0, scaling: Optional[str] = N
 
 def _rope_rows(x):
     """x (B,L,H,D) as the kernel reads it: any strides over a dense last dimension, first element on a 16-byte boundary."""
-    if x.stride(-1) != 1 and x.shape[-1] > 1 or x.data_ptr() % 16:
+    if x.stride(-1) != 1 and x.shape[-1] > 1 or x.data_ptr() & 15:
         x = x.contiguous()
-        if x.data_ptr() % 16:
+        if x.data_ptr() & 15:
             x = x.clone()
     return x
 
 
-def _rope_call(name, sides, pos, inv_freq, interleaved, scaling, eps, w_dtype, ws=None):
-    """sides: (x or None, weight, out, d_out, d_weight) of each tensor."""
-    B, L, _, D = sides[0][2].shape
-    none = (0, 0, 0)
-    t = (_lib.RopeTensor * len(sides))(*[
-        (ptr(x), ptr(w), ptr(out), ptr(g), ptr(dw), *(none if x is None else x.stride()[:3]), *(none if g is None else g.stride()[:3]),
-         out.shape[2], 0) for x, w, out, g, dw in sides])
+_NO_STRIDES = (0, 0, 0)
+
+
+def _rope_side(x, w, out, g=None, dw=None):
+    return (ptr(x), ptr(w), ptr(out), ptr(g), ptr(dw), *(_NO_STRIDES if x is None else x.stride()[:3]),
+            *(_NO_STRIDES if g is None else g.stride()[:3]), out.shape[2], 0)
+
+
+def _rope_call(name, sides, shape, dt, pos, inv_freq, interleaved, scaling, eps, w_dtype, ws=None):
+    """sides: (x or None, weight, out, d_out, d_weight) of each tensor; shape: (B, L, heads, D) of one of them."""
+    t = (_lib.RopeTensor * len(sides))(*sides)
     pb, pl = (0, pos.stride(0)) if pos.dim() == 1 else pos.stride()
     if pos.dim() == 2 and pos.shape[0] == 1:
         pb = 0
-    args = (t, len(sides), ptr(pos) if pos.numel() else None, pos.dtype == torch.int64, pb, pl, ptr(inv_freq), 2 * inv_freq.shape[0], B, L, D,
-            interleaved, scaling, eps, dtype_code(sides[0][2]), w_dtype)
+    args = (t, len(sides), ptr(pos) if pos.numel() else None, pos.dtype == torch.int64, pb, pl, ptr(inv_freq), 2 * inv_freq.shape[0],
+            shape[0], shape[1], shape[3], interleaved, scaling, eps, dt, w_dtype)
     if ws is not None:
         args += (ptr(ws), ws.numel())
     call(name, *args, stream())
 
 
 def _rope_forward(q, k, q_weight, k_weight, positions, inv_freq, interleaved, scaling, eps):
-    """(inputs as read, weights, outputs, type of the weights) of the tensors given."""
-    xs = [_rope_rows(q)] if k is None else [_rope_rows(q), _rope_rows(k)]
-    ws = (q_weight, k_weight)
-    outs = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
-    w = q_weight if q_weight is not None else (k_weight if k is not None else None)
+    """(inputs as read, outputs, type of the weights) of the tensors given."""
+    x = _rope_rows(q)
+    out = x.new_empty(x.shape)
+    xs, outs, sides = [x], [out], [_rope_side(x, q_weight, out)]
+    if k is not None:
+        x = _rope_rows(k)
+        out = x.new_empty(x.shape)
+        xs.append(x), outs.append(out), sides.append(_rope_side(x, k_weight, out))
+    w = q_weight if q_weight is not None else k_weight
     w_dtype = F32 if w is None else dtype_code(w)
-    _rope_call("hils_qk_norm_rope_fwd", [(x, w, o, None, None) for x, w, o in zip(xs, ws, outs)], positions, inv_freq, interleaved, scaling, eps,
-               w_dtype)
-    return xs, ws, outs, w_dtype
+    _rope_call("hils_qk_norm_rope_fwd", sides, q.shape, dtype_code(q), positions, inv_freq, interleaved, scaling, eps, w_dtype)
+    return xs, outs, w_dtype
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, interleaved, scaling, eps):
-        xs, ws, outs, w_dtype = _rope_forward(q, k, q_weight, k_weight, positions, inv_freq, interleaved, scaling, eps)
+        xs, outs, w_dtype = _rope_forward(q, k, q_weight, k_weight, positions, inv_freq, interleaved, scaling, eps)
+        ws = (q_weight, k_weight)[:len(xs)]
         # without a norm the backward is the rotation back, which does not read x
         ctx.save_for_backward(positions, inv_freq, *[t for x, w in zip(xs, ws) if w is not None for t in (x, w)])
-        ctx.meta = ([w is not None for _, w in zip(xs, ws)], [(x.shape, x.dtype) for x in xs], interleaved, scaling, eps, w_dtype)
+        ctx.meta = ([w is not None for w in ws], [(x.shape, x.dtype) for x in xs], interleaved, scaling, eps, w_dtype)
         return outs[0], (outs[1] if k is not None else None)
 
     @staticmethod
@@ -860,18 +875,20 @@ class _QkNormRope(torch.autograd.Function):
         weighted, like, interleaved, scaling, eps, w_dtype = ctx.meta
         positions, inv_freq, *saved = ctx.saved_tensors
         given = iter(saved)
-        grads, d_ws, sides = [None, None], [None, None], []
+        grads, d_ws, sides, held = [None, None], [None, None], [], []
         for i, (has, (shape, dtype), g) in enumerate(zip(weighted, like, (d_q, d_k))):
             x, w = (next(given), next(given)) if has else (None, None)
             if not (ctx.needs_input_grad[i] or ctx.needs_input_grad[2 + i]):
                 continue
-            grads[i] = torch.empty(shape, dtype=dtype, device=positions.device)
+            g = _rope_rows(g if g.dtype == dtype else g.to(dtype))
+            held.append(g)                                     # what the call reads stays alive until it is queued
+            grads[i] = g.new_empty(shape)
             d_ws[i] = None if w is None else torch.empty_like(w)
-            sides.append((x, w, grads[i], _rope_rows(g.to(dtype)), d_ws[i]))
+            sides.append(_rope_side(x, w, grads[i], g, d_ws[i]))
         if sides:
-            ws_bytes = query("hils_qk_norm_rope_bwd_workspace_bytes", like[0][0][-1]) if any(weighted) else 0
-            tmp = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=positions.device)
-            _rope_call("hils_qk_norm_rope_bwd", sides, positions, inv_freq, interleaved, scaling, eps, w_dtype, tmp)
+            ws_bytes = query("hils_qk_norm_rope_bwd_workspace_bytes", like[0][0][-1]) if any(weighted) else 16
+            tmp = held[0].new_empty(ws_bytes, dtype=torch.uint8)
+            _rope_call("hils_qk_norm_rope_bwd", sides, like[0][0], dtype_code(held[0]), positions, inv_freq, interleaved, scaling, eps, w_dtype, tmp)
         return (*grads, *d_ws, None, None, None, None, None)
 
 
@@ -885,25 +902,33 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: f
     rot <= D, the elements behind it are not rotated; pairs are (i, i + rot/2), interleaved (2i, 2i + 1).  q_weight, k_weight
     (D,) or None (no norm for that tensor).  Arithmetic in fp32 with one rounding.  Returns (q_out, k_out or None), dense;
     differentiable with respect to q, k and the weights (once)."""
-    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError(f"qk_norm_rope: q (B,L,h_q,D) and k (B,L,h_k,D), got {tuple(q.shape)} and {None if k is None else tuple(k.shape)}")
     B, L, _, D = q.shape
     dtype_code(q)
-    if k is not None and k.dtype != q.dtype:
-        raise TypeError(f"qk_norm_rope: q of {q.dtype}, k of {k.dtype}")
-    if positions.dtype not in (torch.int32, torch.int64):
+    if k is not None:
+        if k.shape != (B, L, k.shape[2], D):
+            raise ValueError(f"qk_norm_rope: q {tuple(q.shape)} and k {tuple(k.shape)}")
+        if k.dtype != q.dtype:
+            raise TypeError(f"qk_norm_rope: q of {q.dtype}, k of {k.dtype}")
+    if positions.dtype != torch.int64 and positions.dtype != torch.int32:
         raise TypeError(f"qk_norm_rope: positions must be int32 or int64, got {positions.dtype}")
-    if positions.shape not in ((L,), (1, L), (B, L)):
+    if positions.shape != (B, L) and positions.shape != (L,) and positions.shape != (1, L):
         raise ValueError(f"qk_norm_rope: positions {tuple(positions.shape)} for {B} x {L} tokens")
-    if inv_freq.dim() != 1 or inv_freq.dtype not in (torch.float32, torch.float64) or 2 * inv_freq.shape[0] > D:
+    if inv_freq.dim() != 1 or 2 * inv_freq.shape[0] > D or inv_freq.dtype not in (torch.float64, torch.float32):
         raise ValueError(f"qk_norm_rope: inv_freq must be (at most {D // 2},) float64 or float32, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
-    weights = [w for w in (q_weight, k_weight if k is not None else None) if w is not None]
-    for w in weights:
-        if w.shape != (D,):
-            raise ValueError(f"qk_norm_rope: a weight of shape {tuple(w.shape)} for heads of {D}")
-    if len(weights) == 2 and weights[0].dtype != weights[1].dtype:
-        raise TypeError(f"qk_norm_rope: weights of {weights[0].dtype} and {weights[1].dtype}")
-    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    if k is None:
+        k_weight = None
+    if q_weight is not None:
+        if q_weight.shape != (D,):
+            raise ValueError(f"qk_norm_rope: a weight of shape {tuple(q_weight.shape)} for heads of {D}")
+        if k_weight is not None and k_weight.dtype != q_weight.dtype:
+            raise TypeError(f"qk_norm_rope: weights of {q_weight.dtype} and {k_weight.dtype}")
+        q_weight = q_weight.contiguous()
+    if k_weight is not None:
+        if k_weight.shape != (D,):
+            raise ValueError(f"qk_norm_rope: a weight of shape {tuple(k_weight.shape)} for heads of {D}")
+        k_weight = k_weight.contiguous()
     if inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous():
         inv_freq = inv_freq.double().contiguous()
     if positions.data_ptr() % 16:
@@ -911,7 +936,7 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: f
     args = (q, k, q_weight, k_weight, positions, inv_freq, bool(interleaved), float(attention_scaling), float(eps))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
         return _QkNormRope.apply(*args)
-    outs = _rope_forward(*args)[2]
+    outs = _rope_forward(*args)[1]
     return outs[0], (outs[1] if k is not None else None)
 
 
