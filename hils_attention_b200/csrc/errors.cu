@@ -33,7 +33,6 @@ int take_status_paged();
 int take_status_pages();
 int take_status_tree();
 int take_status_tree_tc();
-int take_status_tree_mma();
 }  // namespace hils
 
 extern "C" int hils_version(void) { return 100; }
@@ -50,10 +49,9 @@ extern "C" int hils_take_device_status(void) {
   const int g = hils::take_status_pages();
   const int h = hils::take_status_tree();
   const int i = hils::take_status_tree_tc();
-  const int j = hils::take_status_tree_mma();
-  for (const int v : {a, b, c, d, e, f, g, h, i, j})
+  for (const int v : {a, b, c, d, e, f, g, h, i})
     if (v < 0) return -1;
-  for (const int v : {a, b, c, d, e, f, g, h, i, j})
+  for (const int v : {a, b, c, d, e, f, g, h, i})
     if (v != 0) return v;
   return 0;
 }

@@ -5,9 +5,6 @@
 #include <algorithm>
 
 #include "tree_common.cuh"
-#ifndef TREE_MMA_ROWS
-#define TREE_MMA_ROWS 32
-#endif
 
 namespace hils {
 
@@ -253,12 +250,8 @@ static int tree_splits(int64_t ctas, int tiles, int slots) {
   return best;
 }
 
-// Rows of one key head that a CTA takes.  fp32: the CUDA-core kernel's tile.  bf16: up to 32 rows the warp-level kernel
-// (tree_attn_mma.cu), up to 128 and above the tcgen05 kernels with one and two row groups (tree_attn_tc.cu).
-static int tree_cta_rows(int64_t R, int dtype) {
-  if (dtype != HILS_BF16) return kTreeRows;
-  return R <= TREE_MMA_ROWS ? (R <= 16 ? 16 : 32) : (R <= 128 ? 128 : 256);
-}
+// Rows of one key head that a CTA takes: fp32 the CUDA-core kernel's tile, bf16 one or two row groups of tree_attn_tc.cu.
+static int tree_cta_rows(int64_t R, int dtype) { return dtype != HILS_BF16 ? kTreeRows : (R <= 128 ? 128 : 256); }
 
 static TreeParams tree_plan(int B, int n, int h_q, int h_kv, int max_len, int W, int dtype) {
   TreeParams p = {};
@@ -283,13 +276,11 @@ int take_status_tree() {
 }
 
 int tree_tc_launch(const TreeParams& p, int D, int rows_per_cta, cudaStream_t st);   // tree_attn_tc.cu
-int tree_mma_launch(const TreeParams& p, int D, int rows, cudaStream_t st);           // tree_attn_mma.cu
 
 template <typename T, int D>
 static int launch_tree(const TreeParams& p, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
-    const int rows = tree_cta_rows((int64_t)p.n * (p.h_q / p.h_kv), HILS_BF16);
-    if (int rc = rows <= 32 ? tree_mma_launch(p, D, rows, st) : tree_tc_launch(p, D, rows, st)) return rc;
+    if (int rc = tree_tc_launch(p, D, tree_cta_rows((int64_t)p.n * (p.h_q / p.h_kv), HILS_BF16), st)) return rc;
   } else {
     const size_t smem = tree_smem_floats<D>() * sizeof(float);
     cudaFuncSetAttribute(tree_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

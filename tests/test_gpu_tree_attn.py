@@ -340,3 +340,16 @@ def test_empty_calls(hb):
     o, lse, _ = hb.tree_attn_paged(p["q"][:0], p["k"][:0], p["v"][:0], p["kp"], p["vp"], p["table"][:0].cuda(), p["lens"][:0].cuda(), 10,
                                    p["parents"][:0].cuda())
     assert o.shape == (0, 3, 2, 64)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,hq,hk", [(40, 3, 3), (40, 15, 3), (7, 2, 2), (64, 4, 1)])
+def test_the_same_call_gives_the_same_bits(hb, dtype, D, n, hq, hk):
+    """Shares of one and of many tiles, one and two row groups to a CTA: no result may hang on which warp is ahead."""
+    p = _problem(8, n, hq, hk, D, dtype, [1600, 640, 64, 1500, 0, 321, 129, 1000], ["random", "chain"], seed=D)
+    first = _call(hb, p)
+    for _ in range(60):
+        again = _call(hb, p)
+        assert all(torch.equal(a, b) for a, b in zip(first[:2], again[:2]))
+    assert _status() == 0
