@@ -244,22 +244,22 @@ static int tree_splits(int64_t ctas, int tiles, int slots) {
   int best = 1;
   int64_t cost = INT64_MAX;
   for (int s = 1; s <= std::min(tiles, 64); ++s) {
-    const int64_t waves = (ctas * s + slots - 1) / slots, c = waves * ((tiles + s - 1) / s + 4) + (s > 1 ? 4 : 0);
+    const int64_t waves = (ctas * s + slots - 1) / slots, c = waves * ((tiles + s - 1) / s + 8) + (s > 1 ? 4 : 0);
     if (c < cost) { cost = c; best = s; }
   }
   return best;
 }
 
-// Rows of one key head that a CTA takes: fp32 the CUDA-core kernel's tile, bf16 one or two row groups of tree_attn_tc.cu.
-static int tree_cta_rows(int64_t R, int dtype) { return dtype != HILS_BF16 ? kTreeRows : (R <= 128 ? 128 : 256); }
+// Rows of one key head that a CTA takes: fp32 the CUDA-core kernel's tile, bf16 the 128 of a tensor-core instruction.
+static int tree_cta_rows(int dtype) { return dtype == HILS_BF16 ? 128 : kTreeRows; }
 
 static TreeParams tree_plan(int B, int n, int h_q, int h_kv, int max_len, int W, int dtype) {
   TreeParams p = {};
   p.B = B; p.n = n; p.h_q = h_q; p.h_kv = h_kv; p.W = W;
   const int64_t R = (int64_t)n * (h_q / h_kv);
-  const int rows = tree_cta_rows(R, dtype);
+  const int rows = tree_cta_rows(dtype);
   p.row_blocks = (int)((R + rows - 1) / rows);
-  p.splits = tree_splits((int64_t)B * h_kv * p.row_blocks, tree_tiles(max_len, W), rows == 256 ? 148 : 148 * 2);
+  p.splits = tree_splits((int64_t)B * h_kv * p.row_blocks, tree_tiles(max_len, W), 148 * 2);
   return p;
 }
 
@@ -275,12 +275,12 @@ int take_status_tree() {
   return v;
 }
 
-int tree_tc_launch(const TreeParams& p, int D, int rows_per_cta, cudaStream_t st);   // tree_attn_tc.cu
+int tree_tc_launch(const TreeParams& p, int D, cudaStream_t st);   // tree_attn_tc.cu
 
 template <typename T, int D>
 static int launch_tree(const TreeParams& p, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
-    if (int rc = tree_tc_launch(p, D, tree_cta_rows((int64_t)p.n * (p.h_q / p.h_kv), HILS_BF16), st)) return rc;
+    if (int rc = tree_tc_launch(p, D, st)) return rc;
   } else {
     const size_t smem = tree_smem_floats<D>() * sizeof(float);
     cudaFuncSetAttribute(tree_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

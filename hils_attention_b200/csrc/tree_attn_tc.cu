@@ -1,6 +1,6 @@
 // Attention of a tree of drafted tokens over the paged store on the tensor cores (tcgen05 + TMEM + TMA), bf16.
 //
-// One CTA owns 128 or 256 (node, head) rows of one key head and a share of the 64-key tiles (tree_common.cuh: tile 0 is the
+// One CTA owns 128 (node, head) rows of one key head and a share of the 64-key tiles (tree_common.cuh: tile 0 is the
 // drafted nodes, the others are pages).  A page of one head is a contiguous 64 x D block, so a tile is one TMA box per 64
 // columns and the page table costs one 4-byte read per tile.  S = Q K^T goes to tensor memory (two buffers, so the next
 // product runs under this tile's softmax), a thread owns a row of S, P = exp2(S - m), bf16, goes back over the columns its S
@@ -31,13 +31,12 @@ using namespace umma;
 
 constexpr float kTtSlack = 8.f;              // log2 units a row's maximum may grow before O is rescaled
 
-// TG groups of 128 rows share the tiles of a CTA.  One group: two CTAs per SM.  Two groups (more than 128 rows per key head):
-// one CTA per SM, every tile is brought once for 256 rows.  KS, VS: places for the K and the V of a tile.
-template <int D, int TG> struct TtShape {
+// Two CTAs share an SM.  KS, VS: places for the K and the V of a tile.
+template <int D> struct TtShape {
   static constexpr int DB = D / 64, QBYTES = DB * 16384, TBYTES = DB * 8192;
-  static constexpr int KS = TG == 1 ? (D == 128 ? 2 : 4) : (D == 128 ? 5 : 6), VS = TG == 1 ? (D == 128 ? 3 : 4) : (D == 128 ? 5 : 6);
-  static constexpr int THREADS = 128 * TG + 32 * TG + 32;  // row warps, a warp that issues a group's products each, one that brings the tiles
-  static constexpr int VAT = TG * QBYTES + KS * TBYTES, BARS = VAT + VS * TBYTES;
+  static constexpr int KS = D == 128 ? 2 : 4, VS = D == 128 ? 3 : 4;
+  static constexpr int THREADS = 192;                      // row warps, a warp that issues the products, one that brings the tiles
+  static constexpr int VAT = QBYTES + KS * TBYTES, BARS = VAT + VS * TBYTES;
   // The ancestors are worked out where the third V tile will be: it is sent for when they are known.
   static constexpr int SCRATCH = VAT + 2 * TBYTES, SMEM = BARS + 512;
 };
@@ -88,15 +87,15 @@ __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_
       : "memory");
 }
 
-template <int D, int TG>
-__global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree_attn_tc_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
+template <int D>
+__global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ CUtensorMap tmK,
                                                                      const __grid_constant__ CUtensorMap tmV) {
-  using Sh = TtShape<D, TG>;
-  constexpr int KS = Sh::KS, VS = Sh::VS, DB = Sh::DB, TB = Sh::TBYTES, QB = Sh::QBYTES, kRows = 128 * TG, kThreads = Sh::THREADS;
-  constexpr int kMmaWarp = 4 * TG, kLoadWarp = 5 * TG, kTmem = TG == 1 ? 256 : 512;
+  using Sh = TtShape<D>;
+  constexpr int KS = Sh::KS, VS = Sh::VS, DB = Sh::DB, TB = Sh::TBYTES, kRows = 128, kThreads = Sh::THREADS;
+  constexpr int kMmaWarp = 4, kLoadWarp = 5, kTmem = 256;
   extern __shared__ uint8_t tt_smem[];
   uint8_t* Qs = tt_smem;
-  uint8_t* Ks = Qs + TG * QB;
+  uint8_t* Ks = Qs + Sh::QBYTES;
   uint8_t* Vs = tt_smem + Sh::VAT;
   uint64_t* bars = reinterpret_cast<uint64_t*>(tt_smem + Sh::BARS);
   uint64_t* k_full = bars;                 // [KS]
@@ -104,11 +103,11 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
   uint64_t* v_full = k_free + KS;          // [VS]
   uint64_t* v_ready = v_full + VS;         // [VS] and cleared of what nobody sees
   uint64_t* v_free = v_ready + VS;         // [VS]
-  uint64_t* s_full = v_free + VS;          // [TG][2]
-  uint64_t* p_full = s_full + 2 * TG;      // [TG][2]: a warp may be a tile ahead of another, not two
-  uint64_t* pv_done = p_full + 2 * TG;     // [TG]
-  uint64_t* done = pv_done + TG;           // [TG] used once: the group's last product
-  uint64_t* setup = done + TG;             // [1]
+  uint64_t* s_full = v_free + VS;          // [2]
+  uint64_t* p_full = s_full + 2;           // [2]: a warp may be a tile ahead of another, not two
+  uint64_t* pv_done = p_full + 2;          // [1]
+  uint64_t* done = pv_done + 1;            // [1] used once: the last product
+  uint64_t* setup = done + 1;              // [1]
   u64t* bad_s = reinterpret_cast<u64t*>(setup + 1);   // [3] keys with non-finite values: drafts, tiles c0, c0 + 1
   volatile int* tile_ok = reinterpret_cast<volatile int*>(bad_s + 3);   // [8]
   uint32_t& tmem_base_s = *reinterpret_cast<uint32_t*>(const_cast<int*>(tile_ok) + 8);
@@ -123,17 +122,43 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
   bool over;
   const int len = tree_length(p, b, over);
   const int parent = tree_parent(p.parents + (int64_t)b * p.n, p.n, tid);
-  if (tid == 32 * kLoadWarp) {
-    for (int s = 0; s < KS; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_free[s], TG); }
-    for (int s = 0; s < VS; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_ready[s], 1); mbar_init(&v_free[s], TG); }
-    for (int g = 0; g < TG; ++g) {
-      mbar_init(&s_full[2 * g], 1);
-      mbar_init(&s_full[2 * g + 1], 1);
-      mbar_init(&p_full[2 * g], 128);
-      mbar_init(&p_full[2 * g + 1], 128);
-      mbar_init(&pv_done[g], 1);
-      mbar_init(&done[g], 1);
+  // all loads that need no length are sent for first: the rows (a warp its 32, whole rows at a time), the drafted keys and values
+  const int64_t new0 = (int64_t)b * p.n;
+  const int row = rb * kRows + tid;
+  const bool valid = tid < kRows && row < R, draft = split == 0;
+  const int64_t out = valid ? (new0 + row / G) * p.h_q + h * G + row % G : 0;
+  const bf16* kn = static_cast<const bf16*>(p.k_new) + (new0 * p.h_kv + h) * D;
+  const bf16* vn = static_cast<const bf16*>(p.v_new) + (new0 * p.h_kv + h) * D;
+  const int64_t nrs = (int64_t)p.h_kv * D;
+  constexpr int kMeet = kThreads - 32, kDraft = (64 * (D / 8) + kMeet - 1) / kMeet;
+  uint4 qv[D / 8], kx[kDraft], vx[kDraft];
+  if (tid < kRows) {
+    const uint32_t real = __ballot_sync(0xffffffffu, valid);
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      const int x = i * 32 + lane, rr = x / (D / 8), c = x % (D / 8);
+      const int64_t from = __shfl_sync(0xffffffffu, out, rr);
+      qv[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (real >> rr & 1u) qv[i] = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + from * D + c * 8);
     }
+  }
+  if (draft && warp != kLoadWarp) {
+#pragma unroll
+    for (int i = 0; i < kDraft; ++i) {
+      const int x = i * kMeet + tid, r = x / (D / 8), c = x % (D / 8);
+      kx[i] = vx[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < p.n) {
+        kx[i] = *reinterpret_cast<const uint4*>(kn + r * nrs + c * 8);
+        vx[i] = *reinterpret_cast<const uint4*>(vn + r * nrs + c * 8);
+      }
+    }
+  }
+  if (tid == 32 * kLoadWarp) {
+    for (int s = 0; s < KS; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_free[s], 1); }
+    for (int s = 0; s < VS; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_ready[s], 1); mbar_init(&v_free[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 128); }
+    mbar_init(pv_done, 1);
+    mbar_init(done, 1);
     mbar_init(setup, 1);
     mbar_init_fence();
     abort_s = *const_cast<volatile int*>(&g_tree_tc_expired) != 0;
@@ -143,52 +168,23 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
   if (warp == kMmaWarp) tmem_alloc(&tmem_base_s, kTmem);
   const int lo_min = tree_low(p, len), c0 = lo_min >> 6, c1 = (len + 63) >> 6;
   const int nt = 1 + max(0, c1 - c0), per = (nt + p.splits - 1) / p.splits;
-  const int t0 = split * per;
+  const int t0 = split * per, first = c0 + max(t0, 1) - 1;   // first: chunk of this CTA's first page tile
+  int ids = -1;
+  if (warp == kLoadWarp && first + lane < c1) ids = p.pages[(int64_t)b * p.page_stride + first + lane];
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_base_s, tS = tmem, tO = tmem + 128 * TG;       // S: 2 buffers of 64 columns a group, O: D columns a group
+  const uint32_t tmem = tmem_base_s, tS = tmem, tO = tmem + 128;            // S: two buffers of 64 columns, O: D columns
   const int nit = abort_s ? 0 : max(0, min(nt, t0 + per) - t0);
   __syncthreads();                                         // nobody has set abort_s on the way
 
   // ---- ancestors, rows, drafted keys; the producer is already on its way ------------
-  const int64_t new0 = (int64_t)b * p.n;
-  const int row = rb * kRows + tid;
-  const bool valid = tid < kRows && row < R;
-  const int64_t out = valid ? (new0 + row / G) * p.h_q + h * G + row % G : 0;
-  const bf16* kn = static_cast<const bf16*>(p.k_new) + (new0 * p.h_kv + h) * D;
-  const bf16* vn = static_cast<const bf16*>(p.v_new) + (new0 * p.h_kv + h) * D;
-  const int64_t nrs = (int64_t)p.h_kv * D;
   int lo = 0x7fffffff;
   u64t dmask = 0ull;
   if (warp != kLoadWarp) {
-    constexpr int kMeet = kThreads - 32;
     int (*par)[kTreeMaxNodes] = reinterpret_cast<int (*)[kTreeMaxNodes]>(tt_smem + Sh::SCRATCH);
     u64t (*anc)[kTreeMaxNodes] = reinterpret_cast<u64t (*)[kTreeMaxNodes]>(tt_smem + Sh::SCRATCH + 512);
-    // all loads first: the rows (a warp its 32, whole rows at a time), the drafted keys and values
-    constexpr int kDraft = (64 * (D / 8) + kMeet - 1) / kMeet;
-    const bool draft = t0 == 0 && nit > 0;
-    uint4 qv[D / 8], kx[kDraft], vx[kDraft];
-    if (tid < kRows) {
-      const uint32_t real = __ballot_sync(0xffffffffu, valid);
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const int x = i * 32 + lane, rr = x / (D / 8), c = x % (D / 8);
-        const int64_t from = __shfl_sync(0xffffffffu, out, rr);
-        qv[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (real >> rr & 1u) qv[i] = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + from * D + c * 8);
-      }
-    }
     if (draft) {
-#pragma unroll
-      for (int i = 0; i < kDraft; ++i) {
-        const int x = i * kMeet + tid, r = x / (D / 8), c = x % (D / 8);
-        kx[i] = vx[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < p.n) {
-          kx[i] = *reinterpret_cast<const uint4*>(kn + r * nrs + c * 8);
-          vx[i] = *reinterpret_cast<const uint4*>(vn + r * nrs + c * 8);
-        }
-      }
 #pragma unroll
       for (int i = 0; i < kDraft; ++i) {
         const int x = i * kMeet + tid, r = x / (D / 8), c = x % (D / 8);
@@ -206,7 +202,7 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) {
         const int x = i * 32 + lane, rr = x / (D / 8), c = x % (D / 8);
-        *reinterpret_cast<uint4*>(Qs + (warp >> 2) * QB + (c >> 3) * 16384 + sw128_off((warp & 3) * 32 + rr, c & 7)) = qv[i];
+        *reinterpret_cast<uint4*>(Qs + (c >> 3) * 16384 + sw128_off(warp * 32 + rr, c & 7)) = qv[i];
       }
     }
     tree_ancestors(parent, par, anc, tid, 2, kMeet);
@@ -263,8 +259,7 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
       if (lane == 0) mbar_arrive(&v_ready[s]);
       return got;
     };
-    const int first = c0 + max(t0, 1) - 1;                 // chunk of this CTA's first page tile
-    int ids = 0, pg = 0, prev = 0, k_issued = 0, v_issued = 0;
+    int pg = 0, prev = 0, k_issued = 0, v_issued = 0;
     bool ok = true;
     auto bring = [&](uint64_t* full, uint8_t* tile, const CUtensorMap* map, bool draft, int page) {
       if (draft) return;                                   // written and announced by the other warps
@@ -284,7 +279,7 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
       prev = pg;                                           // page of tile step - 1, whose V is due
       if (step < nit) {
         if (t0 + step > 0) {
-          if (((c - first) & 31) == 0) ids = c + lane < c1 ? p.pages[(int64_t)b * p.page_stride + c + lane] : -1;
+          if (c > first && ((c - first) & 31) == 0) ids = c + lane < c1 ? p.pages[(int64_t)b * p.page_stride + c + lane] : -1;
           pg = __shfl_sync(0xffffffffu, ids, (c - first) & 31);
         } else {
           pg = 0;
@@ -322,23 +317,20 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
       for (int it = max(0, k_issued - KS); it < k_issued; ++it) wait_for(&k_full[it % KS], (it / KS) & 1);   // no copy outlives the CTA
       for (int it = max(0, v_issued - VS); it < v_issued; ++it) wait_for(&v_full[it % VS], (it / VS) & 1);
     }
-  } else if (warp >= kMmaWarp) {
-    // ---- products of one row group.  A warp for each group: one for both spends so long on six barriers a tile, beside busy
-    // row warps, that the tensor pipe waits for it (the widest case 200 us).  The whole warp runs the loop and one elected
-    // lane issues: descriptors then live in uniform registers, where the instruction takes them from. ---------------------
+  } else if (warp == kMmaWarp) {
+    // ---- products.  The whole warp runs the loop and one elected lane issues: descriptors then live in uniform registers,
+    // where the instruction takes them from. ------------------------------------------------------------------------------
     if (nit > 0) {
       constexpr uint32_t idesc_qk = idesc_bf16(128, 64, 0);
       constexpr uint32_t idesc_pv = idesc_bf16(128, D, 1);
-      const int g = warp - kMmaWarp;
-      const uint64_t q_d = desc_sw128(smem_u32(Qs + g * QB), 16, 1024), k_d = desc_sw128(smem_u32(Ks), 16, 1024), v_d = desc_sw128(smem_u32(Vs), 8192, 1024);
-      const uint32_t ts = tS + g * 128, to = tO + g * D;
+      const uint64_t q_d = desc_sw128(smem_u32(Qs), 16, 1024), k_d = desc_sw128(smem_u32(Ks), 16, 1024), v_d = desc_sw128(smem_u32(Vs), 8192, 1024);
       auto issue_qk = [&](int it) {
         if (elect_one()) {
           const uint64_t kb = k_d + (it % KS) * (TB >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            mma_ss(ts + (it & 1) * 64, q_d + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), kb + (((kk >> 2) * 8192 + (kk & 3) * 32) >> 4), idesc_qk, kk > 0);
-          mma_commit(&s_full[2 * g + (it & 1)]);
+            mma_ss(tS + (it & 1) * 64, q_d + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), kb + (((kk >> 2) * 8192 + (kk & 3) * 32) >> 4), idesc_qk, kk > 0);
+          mma_commit(&s_full[it & 1]);
           mma_commit(&k_free[it % KS]);
         }
         __syncwarp();
@@ -351,21 +343,21 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
       for (int it = 0; ok && it < nit; ++it) {
         if (__any_sync(0xffffffffu, abort_s)) break;
         if (it + 1 < nit) {                                // into the columns of S and P of it - 1
-          if (it > 0) ok = wait_for(&pv_done[g], (it - 1) & 1);
+          if (it > 0) ok = wait_for(pv_done, (it - 1) & 1);
           ok = __all_sync(0xffffffffu, ok && wait_for(&k_full[(it + 1) % KS], ((it + 1) / KS) & 1));
           if (!ok) break;
           tc_fence_after();
           issue_qk(it + 1);
         }
         ok = wait_for(&v_ready[it % VS], (it / VS) & 1);
-        ok = __all_sync(0xffffffffu, ok && wait_for(&p_full[2 * g + (it & 1)], (it >> 1) & 1));
+        ok = __all_sync(0xffffffffu, ok && wait_for(&p_full[it & 1], (it >> 1) & 1));
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
           const uint64_t b0 = v_d + (it % VS) * (TB >> 4);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) mma_ts(to, ts + (it & 1) * 64 + kk * 8, b0 + ((kk * 2048) >> 4), idesc_pv, it > 0 || kk > 0);
-          mma_commit(&pv_done[g]);
+          for (int kk = 0; kk < 4; ++kk) mma_ts(tO, tS + (it & 1) * 64 + kk * 8, b0 + ((kk * 2048) >> 4), idesc_pv, it > 0 || kk > 0);
+          mma_commit(pv_done);
           mma_commit(&v_free[it % VS]);
         }
         __syncwarp();
@@ -373,19 +365,18 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
       if (!ok && lane == 0) { abort_s = 1; atomicExch(&g_tree_tc_expired, 8300002); }
       __threadfence_block();
       __syncwarp();
-      if (elect_one()) mma_commit(&done[g]);               // no product outlives the CTA's tensor memory
-      wait_for(&done[g], 0);
+      if (elect_one()) mma_commit(done);               // no product outlives the CTA's tensor memory
+      wait_for(done, 0);
     }
   } else {
     // ---- rows -----------------------------------------------------------------------------------------------------------
-    const int grp = tid >> 7;
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, tSg = tS + grp * 128 + lane_base, tOg = tO + grp * D + lane_base;
+    const uint32_t lane_base = (uint32_t)(warp * 32) << 16, tSg = tS + lane_base, tOg = tO + lane_base;
     const bool rows_here = rb * kRows + warp * 32 < R;
     float m = -CUDART_INF_F, l = 0.f;                      // reference point (log2 units) and sum
     bool ok = true;
     for (int it = 0; it < nit; ++it) {
       const int s = it & 1, t = t0 + it, c = c0 + t - 1;
-      ok = __all_sync(0xffffffffu, wait_for(&s_full[2 * grp + s], (it >> 1) & 1) && !abort_s);
+      ok = __all_sync(0xffffffffu, wait_for(&s_full[s], (it >> 1) & 1) && !abort_s);
       if (!ok) break;
       tc_fence_after();
       float sv[64];
@@ -423,7 +414,7 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
         }
         if (it > 0 && __any_sync(0xffffffffu, moved)) {    // rare after the first tiles: O stands still once the last product is done
           // (never a phase off: S of this tile came after the product of it - 2, the product of `it` waits for this thread)
-          ok = wait_for(&pv_done[grp], (it - 1) & 1) && ok;
+          ok = wait_for(pv_done, (it - 1) & 1) && ok;
           tc_fence_after();
           const float f = moved ? grow : 1.f;
 #pragma unroll 1
@@ -453,12 +444,12 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_before();
-      mbar_arrive(&p_full[2 * grp + s]);
+      mbar_arrive(&p_full[s]);
     }
     // The last product, by a barrier of its own with a single phase.  pv_done cannot be asked here: the products of the last
     // two tiles need nothing more from this thread, so its barrier may be one or two phases ahead of the thread, and a parity
     // does not tell two phases from none.
-    if (ok && nit > 0) ok = __all_sync(0xffffffffu, wait_for(&done[grp], 0) && !abort_s);
+    if (ok && nit > 0) ok = __all_sync(0xffffffffu, wait_for(done, 0) && !abort_s);
     if (!ok && lane == 0) {
       abort_s = 1;
       atomicExch(&g_tree_tc_expired, 8300003);
@@ -481,7 +472,7 @@ __global__ void __launch_bounds__(TtShape<D, TG>::THREADS, TG == 1 ? 2 : 1) tree
         add_bad_keys<D>(p, bad_s, b, h, out, kn, vn, nrs, c0, len, lo, dmask, sl2, m > -CUDART_INF_F ? m : 0.f, cb, ov);
       // through shared memory (Q's place: its last product is done), so that 128 bytes of a row leave together
       if (rows_here) {
-        float4* stage = reinterpret_cast<float4*>(Qs + grp * QB + (warp & 3) * 4096);
+        float4* stage = reinterpret_cast<float4*>(Qs + warp * 4096);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           stage[lane * 8 + (j ^ (lane & 7))] = make_float4(ov[4 * j] * inv, ov[4 * j + 1] * inv, ov[4 * j + 2] * inv, ov[4 * j + 3] * inv);
@@ -524,23 +515,19 @@ int take_status_tree_tc() {
   return x != 0 ? x : v;
 }
 
-template <int D, int TG>
+template <int D>
 static int launch_tree_tc(const TreeParams& p, cudaStream_t st) {
   CUtensorMap tmK, tmV;
   const uint64_t rows = (uint64_t)p.num_pages * p.h_kv * 64;
   if (int rc = make_tmap_bf16_rows(&tmK, p.k_pages, rows, D, D, 64)) return rc;
   if (int rc = make_tmap_bf16_rows(&tmV, p.v_pages, rows, D, D, 64)) return rc;
-  using Sh = TtShape<D, TG>;
-  cudaFuncSetAttribute(tree_attn_tc_kernel<D, TG>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
-  tree_attn_tc_kernel<D, TG><<<dim3((unsigned)(p.row_blocks * p.splits), (unsigned)p.h_kv, (unsigned)p.B), Sh::THREADS, Sh::SMEM, st>>>(p, tmK, tmV);
+  using Sh = TtShape<D>;
+  cudaFuncSetAttribute(tree_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
+  tree_attn_tc_kernel<D><<<dim3((unsigned)(p.row_blocks * p.splits), (unsigned)p.h_kv, (unsigned)p.B), Sh::THREADS, Sh::SMEM, st>>>(p, tmK, tmV);
   HILS_LAUNCH_CHECK("tree_attn_paged (tensor-core path)");
   return HILS_OK;
 }
 
-// rows_per_cta: 128 or 256
-int tree_tc_launch(const TreeParams& p, int D, int rows_per_cta, cudaStream_t st) {
-  if (rows_per_cta == 256) return D == 128 ? launch_tree_tc<128, 2>(p, st) : launch_tree_tc<64, 2>(p, st);
-  return D == 128 ? launch_tree_tc<128, 1>(p, st) : launch_tree_tc<64, 1>(p, st);
-}
+int tree_tc_launch(const TreeParams& p, int D, cudaStream_t st) { return D == 128 ? launch_tree_tc<128>(p, st) : launch_tree_tc<64>(p, st); }
 
 }  // namespace hils
