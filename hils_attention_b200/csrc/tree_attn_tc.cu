@@ -324,43 +324,48 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
       constexpr uint32_t idesc_qk = idesc_bf16(128, 64, 0);
       constexpr uint32_t idesc_pv = idesc_bf16(128, D, 1);
       const uint64_t q_d = desc_sw128(smem_u32(Qs), 16, 1024), k_d = desc_sw128(smem_u32(Ks), 16, 1024), v_d = desc_sw128(smem_u32(Vs), 8192, 1024);
-      auto issue_qk = [&](int it) {
+      auto issue_qk = [&](int buf, int place) {
         if (elect_one()) {
-          const uint64_t kb = k_d + (it % KS) * (TB >> 4);
+          const uint64_t kb = k_d + place * (TB >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            mma_ss(tS + (it & 1) * 64, q_d + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), kb + (((kk >> 2) * 8192 + (kk & 3) * 32) >> 4), idesc_qk, kk > 0);
-          mma_commit(&s_full[it & 1]);
-          mma_commit(&k_free[it % KS]);
+            mma_ss(tS + buf * 64, q_d + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), kb + (((kk >> 2) * 8192 + (kk & 3) * 32) >> 4), idesc_qk, kk > 0);
+          mma_commit(&s_full[buf]);
+          mma_commit(&k_free[place]);
         }
         __syncwarp();
       };
       bool ok = __all_sync(0xffffffffu, wait_for(&k_full[0], 0));
       if (ok) {
         tc_fence_after();
-        issue_qk(0);
+        issue_qk(0, 0);
       }
+      // places and phases are counted along: a division by VS costs as much as a barrier
+      int ks = 0, vs = 0;
+      uint32_t kp = 0, vp = 0;
       for (int it = 0; ok && it < nit; ++it) {
-        if (__any_sync(0xffffffffu, abort_s)) break;
+        const int buf = it & 1;
         if (it + 1 < nit) {                                // into the columns of S and P of it - 1
-          if (it > 0) ok = wait_for(pv_done, (it - 1) & 1);
-          ok = __all_sync(0xffffffffu, ok && wait_for(&k_full[(it + 1) % KS], ((it + 1) / KS) & 1));
-          if (!ok) break;
+          if (++ks == KS) { ks = 0; kp ^= 1; }
+          ok = wait_for(&k_full[ks], kp);
+          if (it > 0) ok = wait_for(pv_done, buf ^ 1) && ok;
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
           tc_fence_after();
-          issue_qk(it + 1);
+          issue_qk(buf ^ 1, ks);
         }
-        ok = wait_for(&v_ready[it % VS], (it / VS) & 1);
-        ok = __all_sync(0xffffffffu, ok && wait_for(&p_full[it & 1], (it >> 1) & 1));
-        if (!ok) break;
+        ok = wait_for(&v_ready[vs], vp);
+        ok = wait_for(&p_full[buf], (it >> 1) & 1) && ok;
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t b0 = v_d + (it % VS) * (TB >> 4);
+          const uint64_t b0 = v_d + vs * (TB >> 4);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) mma_ts(tO, tS + (it & 1) * 64 + kk * 8, b0 + ((kk * 2048) >> 4), idesc_pv, it > 0 || kk > 0);
+          for (int kk = 0; kk < 4; ++kk) mma_ts(tO, tS + buf * 64 + kk * 8, b0 + ((kk * 2048) >> 4), idesc_pv, it > 0 || kk > 0);
           mma_commit(pv_done);
-          mma_commit(&v_free[it % VS]);
+          mma_commit(&v_free[vs]);
         }
         __syncwarp();
+        if (++vs == VS) { vs = 0; vp ^= 1; }
       }
       if (!ok && lane == 0) { abort_s = 1; atomicExch(&g_tree_tc_expired, 8300002); }
       __threadfence_block();
