@@ -79,6 +79,18 @@ __device__ __forceinline__ void add_bad_keys(const TreeParams& p, const u64t* ba
   }
 }
 
+// two fp32 sums or products at a time
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(reinterpret_cast<u64t&>(a)), "l"(reinterpret_cast<u64t&>(b)), "l"(reinterpret_cast<u64t&>(c)));
+  return reinterpret_cast<float2&>(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(reinterpret_cast<u64t&>(a)), "l"(reinterpret_cast<u64t&>(b)));
+  return reinterpret_cast<float2&>(d);
+}
+
 // D[tmem] (+)= A[tmem] * B[smem]; A: 128 rows, two bf16 to a column
 __device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -433,17 +445,20 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
           }
         }
         const float ref = m > -CUDART_INF_F ? m : 0.f;
-        float s4[4] = {0.f, 0.f, 0.f, 0.f}, pk[32];        // pk: pairs of bf16
+        const float2 sl2x2 = make_float2(sl2, sl2), refx2 = make_float2(-ref, -ref);
+        float2 s4[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        float pk[32];                                      // pairs of bf16
 #pragma unroll
         for (int j = 0; j < 64; j += 2) {
-          const float w0 = ex2(fmaf(sv[j], sl2, -ref)), w1 = ex2(fmaf(sv[j + 1], sl2, -ref));   // -inf gives 0
-          s4[j & 3] += w0;
-          s4[(j & 3) + 1] += w1;
-          const __nv_bfloat162 hh = __floats2bfloat162_rn(w0, w1);
+          float2 w = fma2(make_float2(sv[j], sv[j + 1]), sl2x2, refx2);
+          w = make_float2(ex2(w.x), ex2(w.y));             // -inf gives 0
+          s4[j >> 1 & 1] = add2(s4[j >> 1 & 1], w);
+          const __nv_bfloat162 hh = __floats2bfloat162_rn(w.x, w.y);
           pk[j >> 1] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&hh));
         }
         tmem_st32(tSg + s * 64, pk);                       // over the first half of the columns S had
-        l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        const float2 sum = add2(s4[0], s4[1]);
+        l += sum.x + sum.y;
         tmem_st_wait();
       }
       ok = __all_sync(0xffffffffu, ok);
