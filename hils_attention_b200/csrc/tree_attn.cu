@@ -19,8 +19,8 @@ constexpr size_t tree_smem_floats() { return (size_t)kTreeRows * D + 64 * (D + 4
 template <typename T, int D>
 __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeParams p) {
   constexpr int CPT = D / 16;                             // output columns of a thread: float4 at 4 tx, and 64 + 4 tx
-  __shared__ int par_s[2][kTreeMaxNodes];
-  __shared__ u64t anc_s[2][kTreeMaxNodes], vis_s[kTreeRows];
+  __shared__ int par_s[kTreeMaxNodes];
+  __shared__ u64t anc[kTreeMaxNodes + 1], vis_s[kTreeRows];
   __shared__ int lo_s[kTreeRows];
   __shared__ u64t dmask_s[kTreeRows];
   extern __shared__ __align__(16) float tsm[];
@@ -34,14 +34,13 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeParams p) {
   bool over;
   const int len = tree_length(p, b, over);
   if (over && tid == 0) atomicExch(&g_tree_status, 8200002);
-  tree_ancestors(tree_parent(p.parents + (int64_t)b * p.n, p.n, tid), par_s, anc_s, tid, 0, kTreeThreads);
-  const u64t* anc = anc_s[0];
+  tree_ancestors(tree_parents(p.parents + (int64_t)b * p.n, p.n, tid), p.n, len, p.mask_lmk, par_s, anc, tid, 0, kTreeThreads);
   if (tid < kTreeRows) {
     const int row = rb * kTreeRows + tid, j = row / G;
     const bool there = row < R && anc[j] != 0ull;
     const int lo = there ? tree_low(p, len + __popcll(anc[j]) - 1) : 0x7fffffff;
     lo_s[tid] = lo;
-    dmask_s[tid] = there ? tree_draft_mask(p, anc, j, len, lo) : 0ull;
+    dmask_s[tid] = there ? tree_draft_mask(anc, j, len, lo) : 0ull;
   }
   const int64_t new0 = (int64_t)b * p.n;
   for (int x = tid; x < kTreeRows * (D / 4); x += kTreeThreads) {
@@ -225,11 +224,11 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
 
 // Positions of the nodes, -1 for those that are absent.
 __global__ void __launch_bounds__(kTreeMaxNodes) tree_positions_kernel(const int32_t* parents, const int32_t* lens, int32_t* pos, int n) {
-  __shared__ int par_s[2][kTreeMaxNodes];
-  __shared__ u64t anc_s[2][kTreeMaxNodes];
+  __shared__ int par_s[kTreeMaxNodes];
+  __shared__ u64t anc[kTreeMaxNodes + 1];
   const int b = blockIdx.x, j = threadIdx.x;
-  tree_ancestors(tree_parent(parents + (int64_t)b * n, n, j), par_s, anc_s, j, 0, kTreeMaxNodes);
-  if (j < n) pos[(int64_t)b * n + j] = anc_s[0][j] ? max(lens[b], 0) + __popcll(anc_s[0][j]) - 1 : -1;
+  tree_ancestors(tree_parents(parents + (int64_t)b * n, n, j), n, 0, 0, par_s, anc, j, 0, kTreeMaxNodes);
+  if (j < n) pos[(int64_t)b * n + j] = anc[j] ? max(lens[b], 0) + __popcll(anc[j]) - 1 : -1;
 }
 
 // Tiles of a sequence of at most max_len tokens

@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
   const int rb = blockIdx.x % p.row_blocks, split = blockIdx.x / p.row_blocks, h = blockIdx.y, b = blockIdx.z;
   bool over;
   const int len = tree_length(p, b, over);
-  const int parent = tree_parent(p.parents + (int64_t)b * p.n, p.n, tid);
+  const int2 parents = tree_parents(p.parents + (int64_t)b * p.n, p.n, tid);
   // all loads that need no length are sent for first: the rows (a warp its 32, whole rows at a time), the drafted keys and values
   const int64_t new0 = (int64_t)b * p.n;
   const int row = rb * kRows + tid;
@@ -194,8 +194,7 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
   int lo = 0x7fffffff;
   u64t dmask = 0ull;
   if (warp != kLoadWarp) {
-    int (*par)[kTreeMaxNodes] = reinterpret_cast<int (*)[kTreeMaxNodes]>(tt_smem + Sh::SCRATCH);
-    u64t (*anc)[kTreeMaxNodes] = reinterpret_cast<u64t (*)[kTreeMaxNodes]>(tt_smem + Sh::SCRATCH + 512);
+    u64t* anc = reinterpret_cast<u64t*>(tt_smem + Sh::SCRATCH);
     if (draft) {
 #pragma unroll
       for (int i = 0; i < kDraft; ++i) {
@@ -217,10 +216,10 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
         *reinterpret_cast<uint4*>(Qs + (c >> 3) * 16384 + sw128_off(warp * 32 + rr, c & 7)) = qv[i];
       }
     }
-    tree_ancestors(parent, par, anc, tid, 2, kMeet);
-    if (valid && anc[0][row / G] != 0ull) {
-      lo = tree_low(p, len + __popcll(anc[0][row / G]) - 1);
-      dmask = tree_draft_mask(p, anc[0], row / G, len, lo);
+    tree_ancestors(parents, p.n, len, p.mask_lmk, reinterpret_cast<int*>(anc + kTreeMaxNodes + 2), anc, tid, 2, kMeet);
+    if (valid && anc[row / G] != 0ull) {
+      lo = tree_low(p, len + __popcll(anc[row / G]) - 1);
+      dmask = tree_draft_mask(anc, row / G, len, lo);
     }
     named_bar_sync(2, kMeet);
     if (draft && bad_s[0] != 0ull)                         // the other pieces of those rows

@@ -28,30 +28,35 @@ struct TreeParams {
 };
 
 // Ancestors of the tree's nodes.  anc[j]: bits of j and its ancestors, 0 when j is absent: its parent is no earlier node
-// and not -1, or an ancestor is absent.  Pointer doubling: six rounds cover 64 nodes, and a bad parent cannot make it loop.
-// Called by `threads` threads (at least 64, thread 0 among them) that meet at barrier `bar`; parent: that of node tid, which
-// the caller loads early; par and anc: [2][64] in shared memory; the result is in anc[0].
-__device__ __forceinline__ int tree_parent(const int32_t* parents, int n, int tid) { return tid < min(n, kTreeMaxNodes) ? parents[tid] : -2; }
+// and not -1, or an ancestor is absent.  anc[64]: bits of the nodes at landmark positions, if those are masked.  Pointer
+// doubling, log2 n rounds: a bad parent cannot make it loop.  One warp does it, two nodes to a lane (four times as fast as
+// rounds that meet at a barrier).  Called by `threads` threads (thread 0 to 31 among them) that meet at barrier `bar` once at
+// the end; parents: those of nodes tid and tid + 32, which the caller loads early; par [64], anc [65] in shared memory.
+__device__ __forceinline__ int2 tree_parents(const int32_t* parents, int n, int tid) {
+  return make_int2(tid < min(n, 32) ? parents[tid] : -2, tid < min(n, kTreeMaxNodes) - 32 ? parents[tid + 32] : -2);
+}
 
-__device__ __forceinline__ void tree_ancestors(int parent, int (*par)[kTreeMaxNodes], u64t (*anc)[kTreeMaxNodes], int tid, int bar, int threads) {
-  auto meet = [&] { asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads) : "memory"); };
-  if (tid < kTreeMaxNodes) {
-    par[0][tid] = (parent >= -1 && parent < tid) ? parent : -2;      // -2: absent
-    anc[0][tid] = 1ull << tid;
-  }
-  meet();
-#pragma unroll
-  for (int r = 0; r < 6; ++r) {
-    const int a = r & 1;
-    if (tid < kTreeMaxNodes) {
-      const int pj = par[a][tid];
-      par[a ^ 1][tid] = pj >= 0 ? par[a][pj] : pj;
-      anc[a ^ 1][tid] = pj >= 0 ? (anc[a][tid] | anc[a][pj]) : anc[a][tid];
+__device__ __forceinline__ void tree_ancestors(int2 parents, int n, int len, int mask_lmk, int* par, u64t* anc, int tid, int bar, int threads) {
+  if (tid < 32) {
+    int p0 = (parents.x >= -1 && parents.x < tid) ? parents.x : -2, p1 = (parents.y >= -1 && parents.y < tid + 32) ? parents.y : -2;   // -2: absent
+    u64t a0 = 1ull << tid, a1 = 1ull << (tid + 32);
+    for (int far = 1; far < min(n, kTreeMaxNodes); far *= 2) {
+      par[tid] = p0;
+      par[tid + 32] = p1;
+      anc[tid] = a0;
+      anc[tid + 32] = a1;
+      __syncwarp();
+      if (p0 >= 0) { a0 |= anc[p0]; p0 = par[p0]; }
+      if (p1 >= 0) { a1 |= anc[p1]; p1 = par[p1]; }
+      __syncwarp();
     }
-    meet();
+    anc[tid] = p0 == -1 ? a0 : 0ull;
+    anc[tid + 32] = p1 == -1 ? a1 : 0ull;
+    const uint32_t l0 = __ballot_sync(0xffffffffu, mask_lmk && ((len + __popcll(a0) - 1) & 63) == 63);
+    const uint32_t l1 = __ballot_sync(0xffffffffu, mask_lmk && ((len + __popcll(a1) - 1) & 63) == 63);
+    if (tid == 0) anc[kTreeMaxNodes] = (u64t)l1 << 32 | l0;
   }
-  if (tid < kTreeMaxNodes && par[0][tid] != -1) anc[0][tid] = 0ull;
-  meet();
+  asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads) : "memory");
 }
 
 __device__ __forceinline__ int tree_low(const TreeParams& p, int t) {      // leftmost position visible from position t
@@ -62,14 +67,14 @@ __device__ __forceinline__ int tree_low(const TreeParams& p, int t) {      // le
 }
 
 // bits of the drafted nodes that node j sees
-__device__ __forceinline__ u64t tree_draft_mask(const TreeParams& p, const u64t* anc, int j, int len, int lo) {
-  u64t m = anc[j], out = 0ull;
-  for (u64t rest = m; rest; rest &= rest - 1) {
-    const int i = __ffsll((long long)rest) - 1;
-    const int t = len + __popcll(anc[i]) - 1;
-    if (t >= lo && !(p.mask_lmk && (t & 63) == 63)) out |= 1ull << i;
-  }
-  return out;
+__device__ __forceinline__ u64t tree_draft_mask(const u64t* anc, int j, int len, int lo) {
+  u64t m = anc[j] & ~anc[kTreeMaxNodes];
+  if (lo > len)                                           // a window shorter than the path
+    for (u64t rest = m; rest; rest &= rest - 1) {
+      const int i = __ffsll((long long)rest) - 1;
+      if (len + __popcll(anc[i]) - 1 < lo) m &= ~(1ull << i);
+    }
+  return m;
 }
 
 // bits of a page tile's keys (tokens 64c .. 64c + 63) that a row with left edge lo sees
