@@ -216,9 +216,9 @@ class HiLSAttentionCore(torch.nn.Module):
         k_pages, v_pages, table, lens, lmk_k, prior_b = store.step_args(self.layer_idx)
         max_len = max((store.length(b) for b in store.active_slots()), default=0)
         out = ops.decode_tree_paged(q.contiguous(), ld, kd, vd, k_pages, v_pages, table, lens, max_len, parents, lmk_k, prior_b, self.topk,
-                                    self.chunk_size, self.hils_sliding_window, self.enable_softmax1, workspace=getattr(self, "_paged_ws", None),
+                                    self.chunk_size, self.hils_sliding_window, self.enable_softmax1, workspace=getattr(self, "_tree_ws", None),
                                     return_indices=return_indices)
-        self._paged_ws = out[-1]
+        self._tree_ws = out[-1]          # not decode_paged's: a captured step of one kind must not lose its scratch to the other
         return out[:2] if return_indices else out[0]
 
     def pool_accepted(self, store, position_embeddings=None):

@@ -136,7 +136,8 @@ class PagedKVStore:
         self._active: List[bool] = [False] * max_seqs
         self._in_step = False
         self._tree = 0                                              # nodes per sequence of the drafted step in progress
-        self._drafts: Optional[Tuple[torch.Tensor, ...]] = None     # k, v, lmk_q of the drafted tokens of every layer
+        self._drafts: Optional[Tuple[torch.Tensor, ...]] = None     # k, v, lmk_q of the drafted tokens of every layer: views of
+        self._draft_room: Optional[Tuple[torch.Tensor, ...]] = None  # room for max_seqs sequences of the widest tree so far
         self._paths: Optional[List[List[int]]] = None               # accepted nodes per slot, between accept_tree and end_tree
 
     # ---- bookkeeping ---------------------------------------------------------------------------------
@@ -350,15 +351,20 @@ class PagedKVStore:
     # ---- a step over drafted trees -------------------------------------------------------------------
     def begin_tree(self, n: int) -> int:
         """Begin a step over trees of up to `n` drafted tokens per sequence (at most 64) and return max_len.  Every active
-        sequence gets the pages for n more tokens; unused ones stay reserved for its next tokens."""
+        sequence gets the pages for n more tokens; unused ones stay reserved for its next tokens.  The drafts' buffers are kept
+        from step to step and only move when a tree is wider than all before it: begin one of the largest n (and end it with
+        nothing accepted) before a step is captured into a graph."""
         if self._in_step:
             raise RuntimeError("begin_tree() between begin_step() / begin_tree() and its end")
         if not 1 <= n <= 64:
             raise ValueError(f"a tree of {n} nodes (1 to 64)")
         self._reserve({b: n for b in self.active_slots()})
+        heads = (self.h_kv, self.h_kv, self.h_q)
+        room = self.num_layers * self.max_seqs * n * self.D
+        if self._draft_room is None or self._draft_room[0].numel() < room * self.h_kv:
+            self._draft_room = tuple(torch.empty(room * h, dtype=self.dtype, device=self.device) for h in heads)
         shape = (self.num_layers, self.batch, n)
-        if self._drafts is None or self._drafts[0].shape[:3] != shape:
-            self._drafts = tuple(torch.empty((*shape, h, self.D), dtype=self.dtype, device=self.device) for h in (self.h_kv, self.h_kv, self.h_q))
+        self._drafts = tuple(t[:shape[0] * shape[1] * n * h * self.D].view(*shape, h, self.D) for t, h in zip(self._draft_room, heads))
         self._in_step, self._tree, self._paths = True, int(n), None
         return max((self._lens[b] for b in self.active_slots()), default=0)
 

@@ -561,16 +561,17 @@ def tree_attn_paged(q, k_new, v_new, k_pages, v_pages, page_table, lens, max_len
         raise ValueError(f"tree_attn_paged: window_size {window_size} (None for the whole cache)")
     else:
         W = int(window_size)
+    max_len, asked, scale = int(max_len), workspace is None, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    if W >= 1 << 31 or max_len >= 1 << 31:
+        raise ValueError(f"tree_attn_paged: window_size {window_size}, max_len {max_len} do not fit 32 bits")
     o, lse = torch.empty_like(q), q.new_empty((B, n, h_q), dtype=torch.float32)
-    max_len, asked = int(max_len), workspace is None
 
     def size():
         return torch.empty(query("hils_tree_attn_paged_workspace_bytes", B, n, h_q, h_kv, D, max_len, W, dt), dtype=torch.uint8, device=q.device)
     if asked:
         workspace = size()
     args = (ptr(q), ptr(k_new), ptr(v_new), ptr(k_pages), ptr(v_pages), ptr(page_table), page_table.shape[1], pages, ptr(lens), max_len,
-            ptr(parents), ptr(o), ptr(lse), B, n, h_q, h_kv, D, W, chunk_size, 1 if mask_lmk else 0, 1 if expand_to_chunk else 0,
-            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), dt)
+            ptr(parents), ptr(o), ptr(lse), B, n, h_q, h_kv, D, W, chunk_size, 1 if mask_lmk else 0, 1 if expand_to_chunk else 0, scale, dt)
     if not call_or_workspace("hils_tree_attn_paged", *args, ptr(workspace) if workspace.numel() else None, workspace.numel(), stream()):
         workspace = size()
         call("hils_tree_attn_paged", *args, ptr(workspace), workspace.numel(), stream())
@@ -608,18 +609,20 @@ def decode_tree_paged(q, lmk_q, k_new, v_new, k_pages, v_pages, page_table, lens
     for t in (q, lmk_q, k_new, v_new, k_pages, v_pages, page_table, lens, parents, lmk_k):
         if not t.is_contiguous():
             raise ValueError("decode_tree_paged: tensors must be contiguous")
+    topk, max_len, window_size, scale = int(topk), int(max_len), int(window_size), 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    if max(topk, max_len, window_size) >= 1 << 31 or topk < 1:
+        raise ValueError(f"decode_tree_paged: topk {topk}, max_len {max_len}, window_size {window_size}")
     pb = None if prior_b is None else prior_b.to(torch.float32).contiguous()
     if pb is not None and pb.shape != (B, N, h_q):
         raise ValueError(f"decode_tree_paged: prior_b {tuple(pb.shape)}, expected {(B, N, h_q)}")
     o = torch.empty_like(q)
     idx = torch.empty((B, n, h_kv, topk), dtype=torch.int32, device=q.device) if return_indices else None
-    need = query("hils_decode_tree_paged_workspace_bytes", B, n, h_q, h_kv, h_lmk, D, int(topk), N, int(max_len), int(window_size),
-                 int(bool(softmax1)), dt)
+    need = query("hils_decode_tree_paged_workspace_bytes", B, n, h_q, h_kv, h_lmk, D, topk, N, max_len, window_size, int(bool(softmax1)), dt)
     if workspace is None or workspace.numel() < need:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     call("hils_decode_tree_paged", ptr(q), ptr(lmk_q), ptr(k_new), ptr(v_new), ptr(k_pages), ptr(v_pages), ptr(page_table), page_table.shape[1],
-         k_pages.shape[0], ptr(lens), int(max_len), ptr(parents), ptr(lmk_k), ptr(pb), N, ptr(o), ptr(idx), B, n, h_q, h_kv, h_lmk, D, int(topk),
-         int(chunk_size), int(window_size), int(bool(softmax1)), 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), dt,
+         k_pages.shape[0], ptr(lens), max_len, ptr(parents), ptr(lmk_k), ptr(pb), N, ptr(o), ptr(idx), B, n, h_q, h_kv, h_lmk, D, topk,
+         int(chunk_size), window_size, int(bool(softmax1)), scale, dt,
          ptr(workspace) if workspace.numel() else None, workspace.numel(), stream())
     return (o, idx, workspace) if return_indices else (o, workspace)
 

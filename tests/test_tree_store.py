@@ -158,3 +158,41 @@ def test_shapes_and_types_are_refused():
             ops.decode_tree_paged(**{**ok, **change})
     with pytest.raises(RuntimeError):
         ops.decode_tree_paged(**ok)                            # not on a GPU
+
+
+def test_the_drafts_do_not_move_until_a_wider_tree_comes():
+    st = _store()
+    a, b = st.allocate(3), st.allocate(5)
+
+    def step(n):
+        st.begin_tree(n)
+        assert all(t.shape[:3] == (2, st.batch, n) and t.is_contiguous() for t in st._drafts)
+        at = [t.data_ptr() for t in st._drafts]
+        st.accept_tree([[]] * st.batch)
+        st.end_tree()
+        return at
+    first = step(9)
+    assert step(4) == first and step(9) == first
+    st.release(b)
+    assert step(9) == first
+    c = st.allocate(1)
+    st.fork(a)
+    assert c == b and st.batch == 3 and step(9) == first           # all slots
+    step(10)
+    assert st.lens.tolist() == [3, 1, 3]
+
+
+def test_sizes_past_32_bits_are_refused():
+    """They would reach the library with their upper bits cut off."""
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    ok = dict(q=torch.zeros(2, 3, 4, 64), k_new=torch.zeros(2, 3, 2, 64), v_new=torch.zeros(2, 3, 2, 64), k_pages=torch.zeros(5, 2, 64, 64),
+              v_pages=torch.zeros(5, 2, 64, 64), page_table=i32(2, 4), lens=i32(2), max_len=100, parents=i32(2, 3))
+    step = dict(ok, lmk_q=ok["q"], lmk_k=torch.zeros(2, 4, 2, 64), prior_b=None, topk=2)
+    for change in (dict(window_size=2 ** 32 + 1), dict(max_len=2 ** 32 + 1)):
+        with pytest.raises(ValueError, match="max_len"):
+            ops.tree_attn_paged(**{**ok, **change})
+        with pytest.raises(ValueError, match="max_len"):
+            ops.decode_tree_paged(**{**step, **change})
+    for topk in (0, -1, 2 ** 32 + 1):
+        with pytest.raises(ValueError, match="topk"):
+            ops.decode_tree_paged(**{**step, "topk": topk})
