@@ -86,3 +86,9 @@ def test_the_c_entry_points_refuse_bad_arguments():
     assert _call(True, ws=C.c_void_p(0x2004), ws_bytes=need)[0] == WORKSPACE
     assert _lib.load().hils_qk_norm_rope_bwd_workspace_bytes(300) == 0
     assert _call(False, L=0)[0] == 0 and _call(False, heads=(0, 0))[0] == 0
+
+
+def test_the_packed_tensor_is_the_header_s():
+    from hils_attention_b200 import ops
+    x = list(range(1, 14))
+    assert ops._ROPE_TENSOR.pack(*x) == bytes(_lib.RopeTensor(*x))
