@@ -382,25 +382,28 @@ __global__ void __launch_bounds__(kQkThreads, 2) qk_norm_rope_kernel(const __gri
   }
 }
 
-// dw = the sum of the CTAs' shares, in a fixed order: warp w takes the rows w, w + 8, ..., then the warps are added up
+// dw = the sum of the CTAs' shares, in a fixed order: warp w takes the rows w, w + 32, ..., then the warps are added up
+// (32 warps: all loads of a thread are on their way at once)
 struct QkSumParams {
   const float* part[2]; void* dw[2];
   int rows[2];
   int D, out_f32;
 };
 
-__global__ void __launch_bounds__(256) qk_weight_grad_kernel(QkSumParams p) {
-  __shared__ float s[8][33];
+__global__ void __launch_bounds__(1024) qk_weight_grad_kernel(QkSumParams p) {
+  __shared__ float s[32][33];
   const int si = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = blockIdx.x * 32 + lane;
   float acc = 0.f;
   if (d < p.D)
-    for (int r = warp; r < p.rows[si]; r += 8) acc += p.part[si][(int64_t)r * p.D + d];
+#pragma unroll 5
+    for (int r = warp; r < p.rows[si]; r += 32) acc += p.part[si][(int64_t)r * p.D + d];
   s[warp][lane] = acc;
   __syncthreads();
-  if (warp == 0 && d < p.D) {
-    for (int w = 1; w < 8; ++w) acc += s[w][lane];
-    if (p.out_f32) static_cast<float*>(p.dw[si])[d] = acc;
-    else static_cast<bf16*>(p.dw[si])[d] = __float2bfloat16_rn(acc);
+  acc = warp_sum(s[lane][warp]);
+  const int at = blockIdx.x * 32 + warp;
+  if (lane == 0 && at < p.D) {
+    if (p.out_f32) static_cast<float*>(p.dw[si])[at] = acc;
+    else static_cast<bf16*>(p.dw[si])[at] = __float2bfloat16_rn(acc);
   }
 }
 
@@ -527,7 +530,7 @@ static int qk_run(const hils_rope_tensor* t, int n, const void* positions, int p
   }
   if (sums > 0) {
     sum.D = D; sum.out_f32 = weight_dtype == HILS_F32;
-    qk_weight_grad_kernel<<<dim3((unsigned)((D + 31) / 32), (unsigned)sums), 256, 0, st>>>(sum);
+    qk_weight_grad_kernel<<<dim3((unsigned)((D + 31) / 32), (unsigned)sums), 1024, 0, st>>>(sum);
     HILS_LAUNCH_CHECK(what);
   }
   return HILS_OK;

@@ -34,7 +34,44 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeParams p) {
   bool over;
   const int len = tree_length(p, b, over);
   if (over && tid == 0) atomicExch(&g_tree_status, 8200002);
-  tree_ancestors(tree_parents(p.parents + (int64_t)b * p.n, p.n, tid), p.n, len, p.mask_lmk, par_s, anc, tid, 0, kTreeThreads);
+  const int2 parents = tree_parents(p.parents + (int64_t)b * p.n, p.n, tid);
+  const int64_t new0 = (int64_t)b * p.n;
+  constexpr int kQ = kTreeRows * (D / 4) / kTreeThreads, kKv = 64 * (D / 4) / kTreeThreads;
+  float4 qf[kQ], kf[kKv], vf[kKv];
+#pragma unroll
+  for (int i = 0; i < kQ; ++i) {
+    const int x = tid + i * kTreeThreads, r = x / (D / 4), d = (x - r * (D / 4)) * 4, row = rb * kTreeRows + r;
+    qf[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < R) qf[i] = load4(static_cast<const T*>(p.q) + ((new0 + row / G) * p.h_q + h * G + row % G) * D + d);
+  }
+  const int c0 = tree_low(p, len) >> 6, c1 = (len + 63) >> 6;
+  const int nt = 1 + max(0, c1 - c0), per = (nt + p.splits - 1) / p.splits;
+  const int t0 = split * per, t1 = min(nt, t0 + per);
+  // K and V of a tile travel in registers while the tile before is computed, its page id one tile earlier
+  auto page_of = [&](int t) { return t > 0 && t < t1 ? p.pages[(int64_t)b * p.page_stride + c0 + t - 1] : 0; };
+  int pg = page_of(t0);
+  u64t held = 0ull;                                       // keys of the tile that anybody may see
+  bool in_pool = true;
+  auto fetch = [&](int t) {
+    in_pool = (unsigned)pg < (unsigned)p.num_pages;
+    if (!in_pool && tid == 0) atomicExch(&g_tree_status, 8200001);
+    held = !in_pool ? 0ull : (t == 0 ? (p.n >= 64 ? ~0ull : (1ull << p.n) - 1) : tree_page_mask(p, c0 + t - 1, len, 0));
+    const T* kb = t == 0 ? static_cast<const T*>(p.k_new) + (new0 * p.h_kv + h) * D : static_cast<const T*>(p.k_pages) + ((int64_t)pg * p.h_kv + h) * 64 * D;
+    const T* vb = t == 0 ? static_cast<const T*>(p.v_new) + (new0 * p.h_kv + h) * D : static_cast<const T*>(p.v_pages) + ((int64_t)pg * p.h_kv + h) * 64 * D;
+    const int64_t rs = t == 0 ? (int64_t)p.h_kv * D : D;
+#pragma unroll
+    for (int i = 0; i < kKv; ++i) {
+      const int x = tid + i * kTreeThreads, r = x / (D / 4), d = (x - r * (D / 4)) * 4;
+      kf[i] = vf[i] = make_float4(0.f, 0.f, 0.f, 0.f);    // keys nobody may see hold anything, NaN too
+      if (held >> r & 1ull) {
+        kf[i] = load4(kb + r * rs + d);
+        vf[i] = load4(vb + r * rs + d);
+      }
+    }
+    pg = page_of(t + 1);
+  };
+  if (t0 < t1) fetch(t0);
+  tree_ancestors(parents, p.n, len, p.mask_lmk, par_s, anc, tid, 0, kTreeThreads);
   if (tid < kTreeRows) {
     const int row = rb * kTreeRows + tid, j = row / G;
     const bool there = row < R && anc[j] != 0ull;
@@ -42,16 +79,8 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeParams p) {
     lo_s[tid] = lo;
     dmask_s[tid] = there ? tree_draft_mask(anc, j, len, lo) : 0ull;
   }
-  const int64_t new0 = (int64_t)b * p.n;
-  for (int x = tid; x < kTreeRows * (D / 4); x += kTreeThreads) {
-    const int r = x / (D / 4), d = (x - r * (D / 4)) * 4, row = rb * kTreeRows + r;
-    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row < R) f = load4(static_cast<const T*>(p.q) + ((new0 + row / G) * p.h_q + h * G + row % G) * D + d);
-    *reinterpret_cast<float4*>(q_s + r * D + d) = f;
-  }
-  const int c0 = tree_low(p, len) >> 6, c1 = (len + 63) >> 6;
-  const int nt = 1 + max(0, c1 - c0), per = (nt + p.splits - 1) / p.splits;
-  const int t0 = split * per, t1 = min(nt, t0 + per);
+#pragma unroll
+  for (int i = 0; i < kQ; ++i) *reinterpret_cast<float4*>(q_s + (tid + i * kTreeThreads) * 4) = qf[i];
   const int ty = tid >> 4, tx = tid & 15, sr = tid >> 3, sl = tid & 7;
   float acc[2][CPT], m_run = -CUDART_INF_F, l_run = 0.f;   // m_run, l_run: of row sr, the same in its eight threads
 #pragma unroll
@@ -60,38 +89,26 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeParams p) {
     for (int e = 0; e < CPT; ++e) acc[i][e] = 0.f;
   for (int t = t0; t < t1; ++t) {
     const int c = c0 + t - 1;
-    const int pg = t > 0 ? tree_page(p, b, c) : 0;
-    if (pg < 0) {
-      if (tid == 0) atomicExch(&g_tree_status, 8200001);
-      continue;
-    }
     __syncthreads();
-    if (tid < kTreeRows) vis_s[tid] = t == 0 ? dmask_s[tid] : tree_page_mask(p, c, len, lo_s[tid]);
-    // keys nobody may see hold anything, NaN too: their V rows become zeros
-    const u64t held = t == 0 ? (p.n >= 64 ? ~0ull : (1ull << p.n) - 1) : tree_page_mask(p, c, len, 0);
-    const T* kb = t == 0 ? static_cast<const T*>(p.k_new) + (new0 * p.h_kv + h) * D : static_cast<const T*>(p.k_pages) + ((int64_t)pg * p.h_kv + h) * 64 * D;
-    const T* vb = t == 0 ? static_cast<const T*>(p.v_new) + (new0 * p.h_kv + h) * D : static_cast<const T*>(p.v_pages) + ((int64_t)pg * p.h_kv + h) * 64 * D;
-    const int64_t rs = t == 0 ? (int64_t)p.h_kv * D : D;
-    for (int x = tid; x < 64 * (D / 4); x += kTreeThreads) {
-      const int r = x / (D / 4), d = (x - r * (D / 4)) * 4;
-      float4 kf = make_float4(0.f, 0.f, 0.f, 0.f), vf = kf;
-      if (held >> r & 1ull) {
-        kf = load4(kb + r * rs + d);
-        vf = load4(vb + r * rs + d);
-      }
-      *reinterpret_cast<float4*>(k_s + r * (D + 4) + d) = kf;
-      *reinterpret_cast<float4*>(v_s + r * D + d) = vf;
+    if (tid < kTreeRows) vis_s[tid] = t == 0 ? dmask_s[tid] : (in_pool ? tree_page_mask(p, c, len, lo_s[tid]) : 0ull);
+#pragma unroll
+    for (int i = 0; i < kKv; ++i) {
+      const int x = tid + i * kTreeThreads, r = x / (D / 4), d = (x - r * (D / 4)) * 4;
+      *reinterpret_cast<float4*>(k_s + r * (D + 4) + d) = kf[i];
+      *reinterpret_cast<float4*>(v_s + r * D + d) = vf[i];
     }
+    const u64t tile_held = held;
     __syncthreads();
+    if (t + 1 < t1) fetch(t + 1);
     // scores of rows 2 ty, 2 ty + 1 against keys tx, tx + 16, tx + 32, tx + 48
     float s[2][4] = {};
     for (int d = 0; d < D; d += 4) {
       const float4 qa = *reinterpret_cast<const float4*>(q_s + (2 * ty) * D + d), qb = *reinterpret_cast<const float4*>(q_s + (2 * ty + 1) * D + d);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float4 kf = *reinterpret_cast<const float4*>(k_s + (tx + 16 * i) * (D + 4) + d);
-        s[0][i] = fmaf(qa.x, kf.x, fmaf(qa.y, kf.y, fmaf(qa.z, kf.z, fmaf(qa.w, kf.w, s[0][i]))));
-        s[1][i] = fmaf(qb.x, kf.x, fmaf(qb.y, kf.y, fmaf(qb.z, kf.z, fmaf(qb.w, kf.w, s[1][i]))));
+        const float4 kv = *reinterpret_cast<const float4*>(k_s + (tx + 16 * i) * (D + 4) + d);
+        s[0][i] = fmaf(qa.x, kv.x, fmaf(qa.y, kv.y, fmaf(qa.z, kv.z, fmaf(qa.w, kv.w, s[0][i]))));
+        s[1][i] = fmaf(qb.x, kv.x, fmaf(qb.y, kv.y, fmaf(qb.z, kv.z, fmaf(qb.w, kv.w, s[1][i]))));
       }
     }
 #pragma unroll
@@ -132,7 +149,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeParams p) {
 #pragma unroll
     for (int e = 0; e < CPT; ++e) { acc[0][e] *= ca; acc[1][e] *= cb; }
     const u64t va = vis_s[2 * ty], vbits = vis_s[2 * ty + 1];
-    const bool mixed = va != held || vbits != held;       // a key that one row sees and another does not may hold NaN
+    const bool mixed = va != tile_held || vbits != tile_held;       // a key that one row sees and another does not may hold NaN
     for (int key = 0; key < 64; ++key) {
       const float pa = s_s[(2 * ty) * 65 + key], pb = s_s[(2 * ty + 1) * 65 + key];
       float v[CPT];
@@ -182,39 +199,56 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attn_kernel(TreeParams p) {
   }
 }
 
-// Joins the splits: o = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  One warp per row.
+// Joins the splits: o = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  One warp per row.  A lane holds the weights of two shares
+// (there are at most 64), then D / 4 lanes read a share's row, eight shares on their way at once: one after another, 33 shares
+// took 9.3 us.
+constexpr int kTreeMaxSplits = 64;
+
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
-  const int lane = threadIdx.x & 31;
+  constexpr int LPR = D / 4, SPP = 32 / LPR, UN = 8;      // lanes per share, shares per step
+  const int lane = threadIdx.x & 31, sub = lane / LPR, d = (lane % LPR) * 4;
   const int64_t rows = (int64_t)p.B * p.n * p.h_q, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
-  float top = -CUDART_INF_F;
-  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_ml[2 * (s * rows + row)]);
-  top = warp_max(top);
-  const float ref = top > -CUDART_INF_F ? top : 0.f;
-  float acc[D / 32], l = 0.f;
+  float2 ml[2];
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const int64_t at = s * rows + row;
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
-    if (ml.y == 0.f) continue;                            // nothing visible in this share
-    const float w = exp2f(ml.x - ref);
-    l = fmaf(w, ml.y, l);
+  for (int i = 0; i < 2; ++i) {
+    const int s = lane + 32 * i;
+    ml[i] = s < p.splits ? *reinterpret_cast<const float2*>(p.part_ml + 2 * (s * rows + row)) : make_float2(-CUDART_INF_F, 0.f);
+  }
+  const float top = warp_max(fmaxf(ml[0].x, ml[1].x)), ref = top > -CUDART_INF_F ? top : 0.f;
+  float w[2];
 #pragma unroll
-    for (int e = 0; e < D / 32; e += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(p.part_o + at * D + e * 32 + lane * 2);
-      acc[e] = fmaf(w, x.x, acc[e]);
-      acc[e + 1] = fmaf(w, x.y, acc[e + 1]);
+  for (int i = 0; i < 2; ++i) w[i] = ml[i].y == 0.f ? 0.f : exp2f(ml[i].x - ref);      // 0: nothing visible in this share
+  const float l = warp_sum(fmaf(w[0], ml[0].y, w[1] * ml[1].y));
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < p.splits; s0 += UN * SPP) {
+    float4 x[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int s = s0 + u * SPP + sub;
+      x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s < p.splits) x[u] = *reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * D + d);
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int s = s0 + u * SPP + sub;
+      const float wl = __shfl_sync(0xffffffffu, w[0], s & 31), wh = __shfl_sync(0xffffffffu, w[1], s & 31), ws = s < 32 ? wl : wh;
+      if (ws == 0.f) continue;
+      acc.x = fmaf(ws, x[u].x, acc.x);
+      acc.y = fmaf(ws, x[u].y, acc.y);
+      acc.z = fmaf(ws, x[u].z, acc.z);
+      acc.w = fmaf(ws, x[u].w, acc.w);
     }
   }
-  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-  T* o = static_cast<T*>(p.o) + row * D;
-#pragma unroll
-  for (int e = 0; e < D / 32; e += 2) {
-    o[e * 32 + lane * 2] = from_f<T>(acc[e] * inv);
-    o[e * 32 + lane * 2 + 1] = from_f<T>(acc[e + 1] * inv);
+  if constexpr (SPP == 2) {
+    acc.x += __shfl_xor_sync(0xffffffffu, acc.x, 16);
+    acc.y += __shfl_xor_sync(0xffffffffu, acc.y, 16);
+    acc.z += __shfl_xor_sync(0xffffffffu, acc.z, 16);
+    acc.w += __shfl_xor_sync(0xffffffffu, acc.w, 16);
   }
+  const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+  if (sub == 0) store4(static_cast<T*>(p.o) + row * D + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
   if (lane == 0) {
     const float lse = l > 0.f ? (ref + log2f(l)) * kLn2F : (l == l ? -CUDART_INF_F : l);
     p.lse[row] = lse;
@@ -242,7 +276,7 @@ static int tree_tiles(int max_len, int W) {
 static int tree_splits(int64_t ctas, int tiles, int slots) {
   int best = 1;
   int64_t cost = INT64_MAX;
-  for (int s = 1; s <= std::min(tiles, 64); ++s) {
+  for (int s = 1; s <= std::min(tiles, kTreeMaxSplits); ++s) {
     const int64_t waves = (ctas * s + slots - 1) / slots, c = waves * ((tiles + s - 1) / s + 8) + (s > 1 ? 4 : 0);
     if (c < cost) { cost = c; best = s; }
   }
