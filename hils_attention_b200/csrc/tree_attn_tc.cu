@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
   uint64_t* p_full = s_full + 2;           // [2]: a warp may be a tile ahead of another, not two
   uint64_t* pv_done = p_full + 2;          // [1]
   uint64_t* done = pv_done + 1;            // [1] used once: the last product
-  uint64_t* setup = done + 1;              // [1]
+  uint64_t* setup = done + 1;              // [1] the row warps have read the ancestors
   u64t* bad_s = reinterpret_cast<u64t*>(setup + 1);   // [3] keys with non-finite values: drafts, tiles c0, c0 + 1
   volatile int* tile_ok = reinterpret_cast<volatile int*>(bad_s + 3);   // [8]
   uint32_t& tmem_base_s = *reinterpret_cast<uint32_t*>(const_cast<int*>(tile_ok) + 8);
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
     for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 128); }
     mbar_init(pv_done, 1);
     mbar_init(done, 1);
-    mbar_init(setup, 1);
+    mbar_init(setup, 4);
     mbar_init_fence();
     abort_s = *const_cast<volatile int*>(&g_tree_tc_expired) != 0;
     bad_s[0] = bad_s[1] = bad_s[2] = 0ull;
@@ -216,24 +216,27 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
         *reinterpret_cast<uint4*>(Qs + (c >> 3) * 16384 + sw128_off(warp * 32 + rr, c & 7)) = qv[i];
       }
     }
+    fence_async_smem();
     tree_ancestors(parents, p.n, len, p.mask_lmk, reinterpret_cast<int*>(anc + kTreeMaxNodes + 2), anc, tid, 2, kMeet);
-    if (valid && anc[row / G] != 0ull) {
-      lo = tree_low(p, len + __popcll(anc[row / G]) - 1);
-      dmask = tree_draft_mask(anc, row / G, len, lo);
-    }
-    named_bar_sync(2, kMeet);
-    if (draft && bad_s[0] != 0ull)                         // the other pieces of those rows
+    // behind that barrier the rows and the drafted tile are there
+    if (draft && bad_s[0] != 0ull) {                       // rare: the other pieces of those rows
       for (int x = tid; x < 64 * (D / 8); x += kMeet)
         if (bad_s[0] >> (x / (D / 8)) & 1ull) *reinterpret_cast<uint4*>(tile_at(Vs, x / (D / 8), x % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
-    fence_async_smem();
-    named_bar_sync(2, kMeet);
-    if (tid == 0) {
-      mbar_arrive(setup);
-      if (draft) {                                         // the drafted tile is there
-        mbar_arrive(&k_full[0]);
-        mbar_arrive(&v_full[0]);
-        mbar_arrive(&v_ready[0]);
+      fence_async_smem();
+      named_bar_sync(2, kMeet);
+    }
+    if (draft && tid == 0) {
+      mbar_arrive(&k_full[0]);
+      mbar_arrive(&v_full[0]);
+      mbar_arrive(&v_ready[0]);
+    }
+    if (warp < kMmaWarp) {                                 // the masks while the first product runs; then the ancestors' place is free
+      if (valid && anc[row / G] != 0ull) {
+        lo = tree_low(p, len + __popcll(anc[row / G]) - 1);
+        dmask = tree_draft_mask(anc, row / G, len, lo);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(setup);
     }
   }
 
