@@ -15,6 +15,7 @@ torch stream and never synchronise with the host.
 """
 from __future__ import annotations
 
+import functools
 import math
 import struct
 from typing import Optional, Tuple
@@ -879,26 +880,38 @@ class _QkNormRope(torch.autograd.Function):
         return outs[0], (outs[1] if k is not None else None)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_q, d_k):
-        weighted, like, interleaved, scaling, eps, w_dtype = ctx.meta
-        positions, inv_freq, *saved = ctx.saved_tensors
-        given = iter(saved)
-        grads, d_ws, sides, held = [None, None], [None, None], [], []
-        for i, (has, (shape, dtype), g) in enumerate(zip(weighted, like, (d_q, d_k))):
-            x, w = (next(given), next(given)) if has else (None, None)
-            if not (ctx.needs_input_grad[i] or ctx.needs_input_grad[2 + i]):
-                continue
-            g = _rope_rows(g if g.dtype == dtype else g.to(dtype))
-            held.append(g)                                     # what the call reads stays alive until it is queued
-            grads[i] = _rope_out(g)
-            d_ws[i] = None if w is None else torch.empty_like(w)
-            sides.append(_rope_side(x, w, grads[i], g, d_ws[i]))
-        if sides:
-            ws_bytes = query("hils_qk_norm_rope_bwd_workspace_bytes", like[0][0][-1]) if any(weighted) else 16
-            tmp = held[0].new_empty(ws_bytes, dtype=torch.uint8)
-            _rope_call("hils_qk_norm_rope_bwd", sides, like[0][0], dtype_code(held[0]), positions, inv_freq, interleaved, scaling, eps, w_dtype, tmp)
-        return (*grads, *d_ws, None, None, None, None, None)
+        # once_differentiable refuses second derivatives; without create_graph there are none to refuse
+        return (_rope_backward_once if torch.is_grad_enabled() else _rope_backward)(ctx, d_q, d_k)
+
+
+@functools.lru_cache(maxsize=None)
+def _rope_workspace_bytes(D):
+    return query("hils_qk_norm_rope_bwd_workspace_bytes", D)
+
+
+def _rope_backward(ctx, d_q, d_k):
+    weighted, like, interleaved, scaling, eps, w_dtype = ctx.meta
+    positions, inv_freq, *saved = ctx.saved_tensors
+    given = iter(saved)
+    grads, d_ws, sides, held = [None, None], [None, None], [], []
+    for i, (has, (shape, dtype), g) in enumerate(zip(weighted, like, (d_q, d_k))):
+        x, w = (next(given), next(given)) if has else (None, None)
+        if not (ctx.needs_input_grad[i] or ctx.needs_input_grad[2 + i]):
+            continue
+        g = _rope_rows(g if g.dtype == dtype else g.to(dtype))
+        held.append(g)                                     # what the call reads stays alive until it is queued
+        grads[i] = _rope_out(g)
+        d_ws[i] = None if w is None else torch.empty_like(w)
+        sides.append(_rope_side(x, w, grads[i], g, d_ws[i]))
+    if sides:
+        ws_bytes = _rope_workspace_bytes(like[0][0][-1]) if any(weighted) else 16
+        tmp = held[0].new_empty(ws_bytes, dtype=torch.uint8)
+        _rope_call("hils_qk_norm_rope_bwd", sides, like[0][0], dtype_code(held[0]), positions, inv_freq, interleaved, scaling, eps, w_dtype, tmp)
+    return (*grads, *d_ws, None, None, None, None, None)
+
+
+_rope_backward_once = once_differentiable(_rope_backward)
 
 
 def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: float = 1e-6, interleaved: bool = False,
