@@ -353,3 +353,13 @@ def test_the_same_call_gives_the_same_bits(hb, dtype, D, n, hq, hk):
         again = _call(hb, p)
         assert all(torch.equal(a, b) for a, b in zip(first[:2], again[:2]))
     assert _status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("n,G", [(3, 200), (1, 129), (2, 1024), (64, 33)])
+def test_many_heads_share_a_key_head(hb, dtype, n, G):
+    """Row blocks that begin and end inside a node."""
+    p = _problem(2, n, G, 1, 64, dtype, [130, 63], ["chain", "random"], seed=n + G)
+    for W in (None, 100):
+        _check(hb, p, W)
+    assert _status() == 0
