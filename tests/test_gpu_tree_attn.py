@@ -363,3 +363,29 @@ def test_many_heads_share_a_key_head(hb, dtype, n, G):
     for W in (None, 100):
         _check(hb, p, W)
     assert _status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_two_calls_at_once(hb, dtype):
+    """Calls on two streams share the SMs and their tensor memory, beside a kernel that uses it too; each has its own workspace."""
+    ps = [_problem(4, 16, 8, 4, 128, dtype, [3000, 1100, 64, 700], ["random"], seed=1), _problem(3, 50, 6, 2, 64, dtype, [900, 2100, 5], ["binary"], seed=2)]
+    x = [torch.randn(1, 1024, 4, 128, device="cuda").to(dtype) for _ in range(3)]
+    alone = [_call(hb, p) for p in ps]
+    swa = hb.flex_attn_tl(*x, window_size=256, chunk_size=64, training=False, mask_lmk=True, expand_to_chunk=True)[0]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    kept = []
+    for _ in range(25):
+        for p, (_, _, ws), s in zip(ps, alone, streams):
+            with torch.cuda.stream(s):
+                kept.append((p is ps[0], _call(hb, p, workspace=ws)))
+        with torch.cuda.stream(streams[2]):
+            kept.append((None, hb.flex_attn_tl(*x, window_size=256, chunk_size=64, training=False, mask_lmk=True, expand_to_chunk=True)))
+    torch.cuda.synchronize()
+    for first, out in kept:
+        if first is None:
+            assert torch.equal(out[0], swa)
+        else:
+            ref = alone[0 if first else 1]
+            assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
+    assert _status() == 0
