@@ -178,6 +178,16 @@ def stream() -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)       # the same handle without building a Stream object per call
 
 
+def capturing(device: torch.device) -> bool:
+    """Whether work queued on the device's current stream goes into a CUDA graph that is being captured."""
+    if device.type != "cuda":
+        return False
+    if device.index is None or torch._C._cuda_getDevice() == device.index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 ERR_WORKSPACE = -4
 
 

@@ -201,11 +201,13 @@ class HiLSAttentionCore(torch.nn.Module):
         o = o.unsqueeze(1)
         return (o, out[1].unsqueeze(1)) if return_indices else o
 
-    def decode_tree_paged(self, q, k, v, lmk_q, store, parents, return_indices: bool = False):
+    def decode_tree_paged(self, q, k, v, lmk_q, store, parents, return_indices: bool = False, max_len: Optional[int] = None):
         """Drafted trees of all sequences against a paged store: q, lmk_q (B, n, h_q, D), k, v (B, n, h_kv, D) with B =
         store.batch and n as given to store.begin_tree(n); parents (B, n) int32 on the device (ops.tree_attn_paged).  The drafted
         tokens are kept in the store's draft buffers.  Returns (B, n, h_q, D).  When it is known which nodes are accepted:
-        store.accept_tree(paths), pool_accepted(store) of every layer, store.end_tree().  Inference only."""
+        store.accept_tree(paths), pool_accepted(store) of every layer, store.end_tree().  max_len: no sequence is longer when
+        the step runs (store.step_bound; a captured step follows the lengths on the device, up to the bound of its capture).
+        Inference only."""
         if not self.enable_prior_query:
             raise NotImplementedError("decode_tree_paged needs enable_prior_query=True (the pooled chunk keys live in the store)")
         kd, vd, ld = store.draft(self.layer_idx)
@@ -214,11 +216,10 @@ class HiLSAttentionCore(torch.nn.Module):
         for place, x in ((kd, k), (vd, v), (ld, lmk_q)):
             place.copy_(x)
         k_pages, v_pages, table, lens, lmk_k, prior_b = store.step_args(self.layer_idx)
-        max_len = max((store.length(b) for b in store.active_slots()), default=0)
-        out = ops.decode_tree_paged(q.contiguous(), ld, kd, vd, k_pages, v_pages, table, lens, max_len, parents, lmk_k, prior_b, self.topk,
-                                    self.chunk_size, self.hils_sliding_window, self.enable_softmax1, workspace=getattr(self, "_tree_ws", None),
+        out = ops.decode_tree_paged(q.contiguous(), ld, kd, vd, k_pages, v_pages, table, lens, store.step_bound(max_len), parents, lmk_k, prior_b,
+                                    self.topk, self.chunk_size, self.hils_sliding_window, self.enable_softmax1, workspace=store.scratch,
                                     return_indices=return_indices)
-        self._tree_ws = out[-1]          # not decode_paged's: a captured step of one kind must not lose its scratch to the other
+        store.keep_scratch(out[-1])
         return out[:2] if return_indices else out[0]
 
     def pool_accepted(self, store, position_embeddings=None):

@@ -29,7 +29,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 
-from . import ops
+from . import _lib, ops
 
 
 class PagePool:
@@ -139,6 +139,8 @@ class PagedKVStore:
         self._drafts: Optional[Tuple[torch.Tensor, ...]] = None     # k, v, lmk_q of the drafted tokens of every layer: views of
         self._draft_room: Optional[Tuple[torch.Tensor, ...]] = None  # room for max_seqs sequences of the widest tree so far
         self._paths: Optional[List[List[int]]] = None               # accepted nodes per slot, between accept_tree and end_tree
+        self._scratch: Optional[torch.Tensor] = None                # of a drafted step, one for all layers
+        self._captured: List[torch.Tensor] = []                     # what captured steps write to: kept as long as the store
 
     # ---- bookkeeping ---------------------------------------------------------------------------------
     @property
@@ -353,7 +355,7 @@ class PagedKVStore:
         """Begin a step over trees of up to `n` drafted tokens per sequence (at most 64) and return max_len.  Every active
         sequence gets the pages for n more tokens; unused ones stay reserved for its next tokens.  The drafts' buffers are kept
         from step to step and only move when a tree is wider than all before it: begin one of the largest n (and end it with
-        nothing accepted) before a step is captured into a graph."""
+        nothing accepted) before a step is captured into a graph.  A captured step replays a step of the same n and batch."""
         if self._in_step:
             raise RuntimeError("begin_tree() between begin_step() / begin_tree() and its end")
         if not 1 <= n <= 64:
@@ -362,6 +364,7 @@ class PagedKVStore:
         heads = (self.h_kv, self.h_kv, self.h_q)
         room = self.num_layers * self.max_seqs * n * self.D
         if self._draft_room is None or self._draft_room[0].numel() < room * self.h_kv:
+            self._retire(*(self._draft_room or ()))
             self._draft_room = tuple(torch.empty(room * h, dtype=self.dtype, device=self.device) for h in heads)
         shape = (self.num_layers, self.batch, n)
         self._drafts = tuple(t[:shape[0] * shape[1] * n * h * self.D].view(*shape, h, self.D) for t, h in zip(self._draft_room, heads))
@@ -374,6 +377,41 @@ class PagedKVStore:
         if not self._tree:
             raise RuntimeError("draft() without begin_tree()")
         return tuple(t[layer] for t in self._drafts)
+
+    def step_bound(self, max_len: Optional[int] = None) -> int:
+        """The max_len a drafted step is given: no sequence may be longer when it runs.  The longest of the present lengths, or
+        the caller's bound; in a step that is being captured, whose replays follow the lengths on the device, all that a page
+        table holds."""
+        now, most = max((self._lens[b] for b in self.active_slots()), default=0), self.max_pages * self.S
+        if max_len is None:
+            return most if _lib.capturing(self.device) else now
+        if not now <= max_len <= most:
+            raise ValueError(f"max_len {max_len}: the longest sequence has {now} tokens and a page table holds {most}")
+        return int(max_len)
+
+    @property
+    def scratch(self) -> Optional[torch.Tensor]:
+        """Scratch of a drafted step.  The layers run one after the other and share it."""
+        return self._scratch
+
+    def keep_scratch(self, scratch: torch.Tensor) -> None:
+        """The scratch a layer's step used, for the next one.  A captured step goes on writing to its scratch and to the drafts'
+        places whenever it is replayed, so these stay allocated when larger ones follow."""
+        if scratch is not self._scratch:
+            if self._scratch is not None:
+                self._retire(self._scratch)
+            self._scratch = scratch
+        if _lib.capturing(self.device):
+            for t in (scratch, *self._draft_room):
+                if all(t is not c for c in self._captured):
+                    self._captured.append(t)
+
+    @staticmethod
+    def _retire(*buffers: torch.Tensor) -> None:
+        """Before buffers are let go: steps may have used them on another stream than the one they were allocated on."""
+        for t in buffers:
+            if t.is_cuda:
+                t.record_stream(torch.cuda.current_stream(t.device))
 
     def accept_tree(self, paths: Sequence[Sequence[int]]) -> None:
         """After all layers ran: the nodes to keep of every row of the batch, from the root of the accepted path on (node ids

@@ -176,3 +176,103 @@ def test_a_captured_tree_step_follows_its_inputs():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(o, call()[0]) and _status() == 0
+
+
+@pytest.mark.parametrize("hq,hk,D,h_lmk", [(8, 2, 128, 8), (8, 2, 64, 2), (16, 2, 128, 2)])
+def test_grouped_heads_over_more_than_one_range_of_chunks(hq, hk, D, h_lmk):
+    """bf16 with room for thousands of chunks streams the chunk keys in ranges of 1024.  A tree of first nodes only: every node
+    against the single-token step with its query, key and value."""
+    from hils_attention_b200 import ops
+    n, N, K8 = 5, 2304, 8
+    lengths = [131072 + 70, 65536 + 640, 40000, 300]
+    B, width = len(lengths), N
+    g = torch.Generator(device="cuda").manual_seed(D + h_lmk)
+    mk = lambda *s: torch.randn(*s, generator=g, device="cuda").to(BF)
+    pages = sum(t // 64 + 1 for t in lengths) + 1
+    order = torch.randperm(pages - 1, generator=torch.Generator().manual_seed(1)).to(torch.int32) + 1
+    table, at = torch.zeros(B, width, dtype=torch.int32), 0
+    for b, t in enumerate(lengths):
+        table[b, :t // 64 + 1] = order[at:at + t // 64 + 1]
+        at += t // 64 + 1
+    table, lens = table.cuda(), torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    kp, vp, lmk = mk(pages, hk, 64, D), mk(pages, hk, 64, D), mk(B, N, h_lmk, D)
+    pb = torch.randn(B, N, hq, generator=g, device="cuda")
+    q, l, k, v = mk(B, n, hq, D), mk(B, n, hq, D), mk(B, n, hk, D), mk(B, n, hk, D)
+    parents = torch.full((B, n), -1, dtype=torch.int32, device="cuda")
+    o, idx, _ = ops.decode_tree_paged(q, l, k, v, kp, vp, table, lens, max(lengths), parents, lmk, pb, K8, 64, W, return_indices=True)
+    far = 0
+    for j in range(n):
+        want, ids, _ = ops.decode_step_paged(*(x[:, j].contiguous() for x in (q, l, k, v)), kp, vp, table, lens, max(lengths), lmk, pb, K8, 64, W,
+                                             return_indices=True)
+        far += int((ids[0] >= 1024).sum())
+        same = (idx[:, j] == ids).all(-1)                       # the window's log-sum-exp decides none of the ids
+        assert bool(same.all()), f"node {j}: {int((~same).sum())} rows selected otherwise"
+        check(o[:, j], want, BF, f"node {j}")
+    assert far > 0 and _status() == 0
+
+
+def _random_sequence(store, T, g):
+    slot = store.allocate(T)
+    mk = lambda *s: torch.randn(*s, generator=g, device="cuda").to(BF)
+    store.write_prefill(slot, 0, mk(T, store.h_kv, store.D), mk(T, store.h_kv, store.D), mk(T // S, store.h_lmk, store.D),
+                        torch.randn(T // S, store.h_q, generator=g, device="cuda"))
+    return slot
+
+
+def test_a_captured_step_replays_at_lengths_its_capture_did_not_have():
+    """Captured while nothing is selectable, replayed past the window and past 1024 selectable chunks (bf16 with room for 512
+    chunks or more streams the chunk keys first), with a second batch size captured and longer eager steps in between."""
+    from hils_attention_b200.kv_store import PagedKVStore
+    hq, hk, D, n = 8, 2, 64, 6
+    core = _core(hq, hk, K, S, W).eval()
+    store = PagedKVStore(2400, 2, 1152, hk, D, hq, dtype=BF, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(4)
+    mk = lambda *s: torch.randn(*s, generator=g, device="cuda").to(BF)
+    x = [mk(2, n, hq, D), mk(2, n, hk, D), mk(2, n, hk, D), mk(2, n, hq, D)]
+    parents = torch.tensor([[-1, 0, 1, 1, 2, -1], [-1, -1, 0, -2, -2, -2]], dtype=torch.int32, device="cuda")
+
+    def call(B, **kw):
+        return core.decode_tree_paged(*(t[:B] for t in x), store, parents[:B], return_indices=True, **kw)
+
+    def in_step(f):
+        store.begin_tree(n)
+        try:
+            return f()
+        finally:
+            store.accept_tree([[]] * store.batch)
+            store.end_tree()
+
+    def capture(B):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(B)
+        return graph, out
+    with torch.no_grad():
+        _random_sequence(store, 100, g)
+        in_step(lambda: call(1))
+        one = in_step(lambda: capture(1))
+        _random_sequence(store, 70, g)
+        two = in_step(lambda: capture(2))
+        store.release(1)
+        for T in (110, 150, 700, 9000, 70000):
+            store.release(0)
+            assert _random_sequence(store, T, g) == 0
+            for B, (graph, out) in ((1, one), (2, two)):
+                if B == 2:
+                    _random_sequence(store, T // 2, g)
+                x[0].neg_()
+
+                def compare():
+                    want = [t.clone() for t in call(B, max_len=store.max_pages * S)]
+                    plain = [t.clone() for t in call(B)]                    # the present lengths: the same selection
+                    for t in out:
+                        t.zero_()
+                    graph.replay()
+                    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), f"{T} tokens, batch {B}"
+                    assert torch.equal(plain[1], want[1])
+                    return want
+                o, idx = in_step(compare)
+                if T >= 70000:
+                    assert int(idx.max()) >= 1024
+            store.release(1)
+    assert _status() == 0

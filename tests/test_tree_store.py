@@ -1,6 +1,8 @@
 """Bookkeeping of a step over drafted trees on CPU tensors (the row writes replaced by plain indexing), and the argument
 checks of the one-call step (no GPU needed)."""
 import ctypes as C
+import gc
+import weakref
 
 import pytest
 import torch
@@ -196,3 +198,92 @@ def test_sizes_past_32_bits_are_refused():
     for topk in (0, -1, 2 ** 32 + 1):
         with pytest.raises(ValueError, match="topk"):
             ops.decode_tree_paged(**{**step, "topk": topk})
+
+
+def _core_step(monkeypatch, bytes_of):
+    """decode_tree_paged of an attention core over a CPU store with the library call replaced: it records the bound and the
+    scratch it is given and wants bytes_of(batch, max_len) of scratch.  Returns (step(store, n, max_len=None, core=0), calls)."""
+    from hils_attention_b200 import attention
+    calls = []
+
+    def library(q, lmk_q, k, v, kp, vp, table, lens, max_len, parents, lmk_k, prior_b, topk, chunk, window, softmax1, workspace=None, return_indices=False):
+        need = bytes_of(q.shape[0], max_len)
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(need, dtype=torch.uint8)
+        calls.append((max_len, weakref.ref(workspace)))
+        return torch.zeros_like(q), workspace
+    monkeypatch.setattr(attention.ops, "decode_tree_paged", library)
+    cores = [attention.HiLSAttentionCore(attention.HiLSAttentionConfig(4, 2, 2, 64, 128)).eval() for _ in range(2)]
+    for i, c in enumerate(cores):
+        c.layer_idx = i
+
+    def step(st, n, max_len=None, core=0):
+        st.begin_tree(n)
+        q, k = torch.zeros(st.batch, n, 4, 8), torch.zeros(st.batch, n, 2, 8)
+        try:
+            kw = {} if max_len is None else dict(max_len=max_len)
+            cores[core].decode_tree_paged(q, k, k, q, st, torch.full((st.batch, n), -1, dtype=torch.int32), **kw)
+        finally:
+            st.accept_tree([[]] * st.batch)
+            st.end_tree()
+    return step, calls
+
+
+def test_a_captured_step_holds_for_all_lengths_a_sequence_may_reach(monkeypatch):
+    """The bound is frozen into the graph, the lengths are not."""
+    step, calls = _core_step(monkeypatch, lambda b, t: 16)
+    st = _store(max_pages=4)
+    st.allocate(100)
+    step(st, 3)
+    assert calls[-1][0] == 100                                 # eager: the present length
+    monkeypatch.setattr(_lib, "capturing", lambda device: True, raising=False)
+    step(st, 3)
+    assert calls[-1][0] == 256
+    step(st, 3, max_len=200)                                   # the caller's bound
+    assert calls[-1][0] == 200
+    monkeypatch.setattr(_lib, "capturing", lambda device: False)
+    for bad in (99, 257, -1):
+        with pytest.raises(ValueError, match="max_len"):
+            step(st, 3, max_len=bad)
+
+
+def test_what_a_captured_step_writes_to_stays_allocated(monkeypatch):
+    """Scratch and drafts of a captured step outlive larger ones: of a longer cache, a larger batch, a wider tree."""
+    step, calls = _core_step(monkeypatch, lambda b, t: 64 * b + t)
+    st = _store(num_pages=20, max_pages=4)
+    st.allocate(10)
+    flag = [True]
+    monkeypatch.setattr(_lib, "capturing", lambda device: flag[0], raising=False)
+    step(st, 3)
+    captured, room = calls[-1][1], [weakref.ref(t) for t in st._draft_room]
+    st.allocate(70)
+    step(st, 3)                                                # a second captured step, of two sequences
+    second = calls[-1][1]
+    flag[0] = False
+    st.allocate(90)
+    for n in (3, 8):
+        step(st, n)
+        step(st, n, max_len=256)
+    larger = calls[-1][1]
+    gc.collect()
+    assert captured() is not None and second() is not None and second() is not captured()
+    assert larger() is st.scratch and larger() is not second() and all(r() is not None for r in room)
+    # one that no graph writes to goes when a larger one comes
+    st2 = _store()
+    st2.allocate(5)
+    step(st2, 2)
+    first = calls[-1][1]
+    step(st2, 2, max_len=100)
+    gc.collect()
+    assert first() is None
+
+
+def test_the_layers_share_one_scratch_and_stores_do_not(monkeypatch):
+    step, calls = _core_step(monkeypatch, lambda b, t: 64)
+    a, b = _store(), _store()
+    for st in (a, b):
+        st.allocate(5)
+        for core in (0, 1):
+            step(st, 2, core=core)
+    got = [r() for _, r in calls]
+    assert got[0] is got[1] is a.scratch and got[2] is got[3] is b.scratch and a.scratch is not b.scratch
