@@ -496,7 +496,8 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
       if (have) {
         tmem_ld32(tOg + cb * 32, ov);
         tmem_ld_wait32(ov);
-      } else {
+      }
+      if (!have || l == 0.f) {                             // a row that sees nothing: its weights are 0, but 0 * V is NaN for an infinite V
 #pragma unroll
         for (int j = 0; j < 32; ++j) ov[j] = 0.f;
       }

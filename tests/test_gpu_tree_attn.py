@@ -389,3 +389,50 @@ def test_two_calls_at_once(hb, dtype):
             ref = alone[0 if first else 1]
             assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
     assert _status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [100, 2000])                     # one share of the tiles, and several
+def test_absent_nodes_stay_zero_beside_infinite_values(hb, dtype, D, T):
+    """A value that every present row sees is infinite: those rows are not finite, absent ones are 0 and -inf all the same."""
+    p = _problem(1, 6, 4, 2, D, dtype, [T], ["short"], seed=9)
+    for s in (5, T - 3):
+        p["vp"][int(p["table"][0, s // 64]), :, s % 64] = INF
+    o, lse, _ = _call(hb, p)
+    there = p["parents"][0] > -2
+    assert not bool(torch.isfinite(o[0, there]).any()) and bool(torch.isfinite(lse[0, there]).all())
+    assert not bool(o[0, ~there].any()) and bool(torch.isneginf(lse[0, ~there]).all())
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("W,T", [(70, 200), (600, 800)])       # one share of the tiles, and several
+@pytest.mark.parametrize("expand,depth", [(False, 2), (False, 59), (False, 62), (True, 0), (True, 2)])
+def test_non_finite_cache_at_the_edge_of_the_window(hb, dtype, D, W, T, expand, depth):
+    """A cached token inside the window of a chain's first nodes and left of the deeper ones' (in the window's first chunk or in
+    its second): rows that see it are spoiled by it, for the others it is not there."""
+    p = _problem(1, 64, 4, 2, D, dtype, [T], ["chain"], seed=D + W)
+    s = T - W + 1 + depth
+    low = torch.tensor([(T + d - W + 1) // 64 * 64 if expand else T + d - W + 1 for d in range(64)])
+    sees = low <= s
+    assert s % 64 != 63 and bool(sees.any()) and not bool(sees.all())
+    o0, l0, _ = _check(hb, p, W, True, expand)
+    pg, at, col = int(p["table"][0, s // 64]), s % 64, D - 3
+    for name, value in (("vp", INF), ("vp", NAN), ("kp", NAN)):
+        r = {**p, name: p[name].clone()}
+        r[name][pg, :, at] = value
+        o, lse, _ = _call(hb, r, W, expand_to_chunk=expand)
+        assert torch.equal(o[0, ~sees], o0[0, ~sees]) and torch.equal(lse[0, ~sees], l0[0, ~sees])
+        assert not bool(torch.isfinite(o[0, sees]).any())
+        assert bool(torch.isnan(lse[0, sees]).all()) if name == "kp" else torch.equal(lse, l0)
+    # one element of the value: the other columns keep to the bound
+    r = {**p, "vp": p["vp"].clone()}
+    r["vp"][pg, :, at, col] = NAN
+    o, lse, _ = _call(hb, r, W, expand_to_chunk=expand)
+    assert torch.equal(o[0, ~sees], o0[0, ~sees]) and bool(torch.isnan(o[0, sees][..., col]).all())
+    ref = _reference(p["q"], p["k"], p["v"], p["kp"], p["vp"], p["table"], p["lens"], p["parents"], W, True, expand, 1 / math.sqrt(D))
+    o[..., col] = ref[0][..., col].to(o)
+    _near((o, lse), ref, dtype)
+    assert _status() == 0
