@@ -21,6 +21,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -956,7 +957,9 @@ def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: f
     if positions.data_ptr() % 16:
         positions = positions.clone()
     args = (q, k, q_weight, k_weight, positions, inv_freq, bool(interleaved), float(attention_scaling), float(eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+    # a forward-mode tangent goes to autograd too, which refuses it; recording gradients or not has no part in that
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4])) or \
+            (forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in args[:4])):
         return _QkNormRope.apply(*args)
     outs = _rope_forward(*args)[1]
     return outs[0], (outs[1] if k is not None else None)

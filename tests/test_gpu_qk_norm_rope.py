@@ -269,3 +269,19 @@ def test_one_rounding_against_the_table_form(hb):
     a, b = new.float().unflatten(-1, (2, D // 2)), old.float().unflatten(-1, (2, D // 2))
     size = a.square().sum(-2, keepdim=True).sqrt()
     assert bool(((a - b).abs() <= 2.5 * 2.0 ** -7 * size + 1e-6).all())
+
+
+def test_forward_mode_is_refused(hb):
+    """No forward-mode formula is offered: a tangent is refused, not dropped, whether or not gradients are recorded."""
+    import torch.autograd.forward_ad as fw
+    q, k, w = torch.randn(1, 3, 2, 64, device="cuda"), torch.randn(1, 3, 1, 64, device="cuda"), torch.ones(64, device="cuda")
+    pos, freq = torch.arange(3, device="cuda"), hb.rope_frequencies(64, device="cuda")[0]
+    plain = hb.qk_norm_rope(q, k, pos, freq, w, w)
+    with fw.dual_level():
+        assert all(torch.equal(a, b) for a, b in zip(hb.qk_norm_rope(q, k, pos, freq, w, w), plain))     # no tangent among them
+        for i, x in enumerate((q, k, w, w)):
+            args = [q, k, w, w]
+            args[i] = fw.make_dual(x, torch.ones_like(x))
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward"):
+                    hb.qk_norm_rope(args[0], args[1], pos, freq, args[2], args[3])
