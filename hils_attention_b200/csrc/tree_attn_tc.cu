@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
         lo = tree_low(p, len + __popcll(anc[row / G]) - 1);
         dmask = tree_draft_mask(anc, row / G, len, lo);
       }
+      fence_async_smem();                                  // the next to write there is a TMA copy
       __syncwarp();
       if (lane == 0) mbar_arrive(setup);
     }
