@@ -211,8 +211,12 @@ class HiLSAttentionCore(torch.nn.Module):
         if not self.enable_prior_query:
             raise NotImplementedError("decode_tree_paged needs enable_prior_query=True (the pooled chunk keys live in the store)")
         kd, vd, ld = store.draft(self.layer_idx)
-        if k.shape != kd.shape or q.shape != ld.shape:
-            raise ValueError(f"decode_tree_paged: q {tuple(q.shape)}, k {tuple(k.shape)}; the step in progress wants {tuple(ld.shape)}, {tuple(kd.shape)}")
+        # copy_ would spread a smaller tensor over heads or sequences, and convert another type
+        for name, x, place in (("q", q, ld), ("lmk_q", lmk_q, ld), ("k", k, kd), ("v", v, vd)):
+            if x.shape != place.shape:
+                raise ValueError(f"decode_tree_paged: {name} {tuple(x.shape)}; the step in progress wants {tuple(place.shape)}")
+            if x.dtype != place.dtype:
+                raise TypeError(f"decode_tree_paged: {name} of {x.dtype}, the store holds {place.dtype}")
         for place, x in ((kd, k), (vd, v), (ld, lmk_q)):
             place.copy_(x)
         k_pages, v_pages, table, lens, lmk_k, prior_b = store.step_args(self.layer_idx)

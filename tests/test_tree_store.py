@@ -287,3 +287,26 @@ def test_the_layers_share_one_scratch_and_stores_do_not(monkeypatch):
             step(st, 2, core=core)
     got = [r() for _, r in calls]
     assert got[0] is got[1] is a.scratch and got[2] is got[3] is b.scratch and a.scratch is not b.scratch
+
+
+def test_drafts_of_another_shape_or_type_are_refused(monkeypatch):
+    """They would be spread over heads or sequences, or converted, on their way into the pages."""
+    from hils_attention_b200 import attention
+    monkeypatch.setattr(attention.ops, "decode_tree_paged", lambda q, *a, **kw: (torch.zeros_like(q), torch.zeros(1, dtype=torch.uint8)))
+    core = attention.HiLSAttentionCore(attention.HiLSAttentionConfig(4, 2, 2, 64, 128)).eval()
+    st = _store()
+    st.allocate(5), st.allocate(70)
+    st.begin_tree(3)
+    for t in st.draft(0):
+        t.fill_(7)
+    ok = dict(q=torch.zeros(2, 3, 4, 8), k=torch.zeros(2, 3, 2, 8), v=torch.zeros(2, 3, 2, 8), lmk_q=torch.zeros(2, 3, 4, 8))
+    parents = torch.full((2, 3), -1, dtype=torch.int32)
+    for name in ok:
+        x = ok[name]
+        for bad in (x[:, :, :1], x[:1], x[:, :1], x[..., :1], x[0], x[:, :2]):
+            with pytest.raises(ValueError, match=f": {name} "):
+                core.decode_tree_paged(**{**ok, name: bad}, store=st, parents=parents)
+        with pytest.raises(TypeError, match=f": {name} "):
+            core.decode_tree_paged(**{**ok, name: x.double()}, store=st, parents=parents)
+    assert all(bool((t == 7).all()) for t in st.draft(0))      # nothing was written
+    core.decode_tree_paged(**ok, store=st, parents=parents)
