@@ -25,6 +25,7 @@
 // Not faster for these: warp-level products, a persistent kernel, keys as the rows of the product (four CTAs an SM), rows dealt
 // to other warps.  Long caches with few rows run at 0.87 of the copy bandwidth (8 x 16000 tokens, 8 key heads: 92 us in a loop).
 #include <algorithm>
+#include <atomic>
 
 #include "tc_rows.cuh"
 #include "tree_common.cuh"
@@ -34,8 +35,20 @@ namespace hils {
 
 // A page outside the pool (8200001), a length past the table (8200002)
 static __device__ int g_tree_tc_status = 0;
-// A wait that ran out (8300001 ..); CTAs that start later see it and write nothing but zeros
+// A wait that ran out (8300001 ..), for the host alone.  g_tree_tc_given_up is the call (TreeParams::call) it happened in: CTAs of
+// that call that start later return zeros at once, other calls have nothing to do with it.
 static __device__ int g_tree_tc_expired = 0;
+static __device__ unsigned g_tree_tc_given_up = 0u;
+
+__device__ __forceinline__ void give_up(const TreeParams& p, int code) {
+  atomicExch(&g_tree_tc_expired, code);
+  atomicExch(&g_tree_tc_given_up, p.call);
+}
+
+// A replay of a captured call has the number of the capture: what an earlier replay left is cleared before it.
+__global__ void tree_tc_begin_kernel(unsigned call) {
+  if (g_tree_tc_given_up == call) g_tree_tc_given_up = 0u;
+}
 
 using namespace umma;
 
@@ -61,7 +74,7 @@ __device__ __forceinline__ bool not_finite8(uint4 x) {     // eight bf16: an exp
 // row `r` of a [64 x D] tile of DB column blocks, piece c of 16 bytes
 __device__ __forceinline__ uint8_t* tile_at(uint8_t* tile, int r, int c) { return tile + (c >> 3) * 8192 + sw128_off(r, c & 7); }
 
-// Shorter than the common limit (about a second): these waits are for copies and products of one tile, microseconds.
+// Fewer polls than the common limit: these waits are for copies and products of one tile, microseconds.
 __device__ __forceinline__ bool wait_for(uint64_t* b, uint32_t parity) { return mbar_wait<1 << 18>(b, parity); }
 
 // What the products left out for one row: the keys whose V rows were zeroed although this row sees them.  Rare (a value that
@@ -136,7 +149,7 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
   volatile int& abort_s = const_cast<volatile int*>(tile_ok)[9];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if ((reinterpret_cast<uintptr_t>(tt_smem) & 1023) != 0) {   // the tiles need the 1 KB alignment of their swizzle
-    if (tid == 0) atomicExch(&g_tree_tc_expired, 8300009);
+    if (tid == 0) give_up(p, 8300009);
     return;
   }
   const int G = p.h_q / p.h_kv, R = p.n * G;
@@ -183,7 +196,7 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
     mbar_init(done, 1);
     mbar_init(setup, 4);
     mbar_init_fence();
-    abort_s = *const_cast<volatile int*>(&g_tree_tc_expired) != 0;
+    abort_s = *const_cast<volatile unsigned*>(&g_tree_tc_given_up) == p.call;
     bad_s[0] = bad_s[1] = bad_s[2] = 0ull;
     if (over) atomicExch(&g_tree_tc_status, 8200002);
   }
@@ -338,7 +351,7 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
       if (!__all_sync(0xffffffffu, ok && !abort_s)) break;
     }
     if (lane == 0) {
-      if (!ok) { abort_s = 1; atomicExch(&g_tree_tc_expired, 8300001); }
+      if (!ok) { abort_s = 1; give_up(p, 8300001); }
       for (int it = max(0, k_issued - KS); it < k_issued; ++it) wait_for(&k_full[it % KS], (it / KS) & 1);   // no copy outlives the CTA
       for (int it = max(0, v_issued - VS); it < v_issued; ++it) wait_for(&v_full[it % VS], (it / VS) & 1);
     }
@@ -392,7 +405,7 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
         __syncwarp();
         if (++vs == VS) { vs = 0; vp ^= 1; }
       }
-      if (!ok && lane == 0) { abort_s = 1; atomicExch(&g_tree_tc_expired, 8300002); }
+      if (!ok && lane == 0) { abort_s = 1; give_up(p, 8300002); }
       __threadfence_block();
       __syncwarp();
       if (elect_one()) mma_commit(done);               // no product outlives the CTA's tensor memory
@@ -485,10 +498,11 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
     if (ok && nit > 0) ok = __all_sync(0xffffffffu, wait_for(done, 0) && !abort_s);
     if (!ok && lane == 0) {
       abort_s = 1;
-      atomicExch(&g_tree_tc_expired, 8300003);
+      give_up(p, 8300003);
     }
     if (ok) tc_fence_after();
     const bool have = ok && nit > 0 && rows_here;
+    if (!have) { m = -CUDART_INF_F; l = 0.f; }             // given up halfway: as a row that sees nothing, in both outputs
     const float inv = p.splits > 1 ? 1.f : (l > 0.f ? 1.f / l : (l == l ? 0.f : l));
     const int64_t at = (int64_t)split * p.B * p.n * p.h_q + out;
 #pragma unroll 1
@@ -498,7 +512,7 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
         tmem_ld32(tOg + cb * 32, ov);
         tmem_ld_wait32(ov);
       }
-      if (!have || l == 0.f) {                             // a row that sees nothing: its weights are 0, but 0 * V is NaN for an infinite V
+      if (l == 0.f) {                                      // a row that sees nothing: its weights are 0, but 0 * V is NaN for an infinite V
 #pragma unroll
         for (int j = 0; j < 32; ++j) ov[j] = 0.f;
       }
@@ -526,7 +540,7 @@ __global__ void __launch_bounds__(TtShape<D>::THREADS, 2) tree_attn_tc_kernel(co
     }
     if (valid) {
       if (p.splits > 1) {
-        *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, have ? l : 0.f);
+        *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, l);
       } else {
         const float lse = l > 0.f ? (m + log2f(l)) * kLn2F : (l == l ? -CUDART_INF_F : l);
         p.lse[out] = lse;
@@ -549,8 +563,14 @@ int take_status_tree_tc() {
   return x != 0 ? x : v;
 }
 
+static std::atomic<unsigned> g_tree_tc_calls{0u};
+
 template <int D>
-static int launch_tree_tc(const TreeParams& p, cudaStream_t st) {
+static int launch_tree_tc(TreeParams p, cudaStream_t st) {
+  while ((p.call = ++g_tree_tc_calls) == 0u) {}            // 0: nobody
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) cudaGetLastError();   // the launch below reports what is wrong with the stream
+  if (capture == cudaStreamCaptureStatusActive) tree_tc_begin_kernel<<<1, 1, 0, st>>>(p.call);
   CUtensorMap tmK, tmV;
   const uint64_t rows = (uint64_t)p.num_pages * p.h_kv * 64;
   if (int rc = make_tmap_bf16_rows(&tmK, p.k_pages, rows, D, D, 64)) return rc;

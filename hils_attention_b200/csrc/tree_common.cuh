@@ -25,6 +25,7 @@ struct TreeParams {
   float* part_o; float* part_ml;       // splits > 1: (split, b, node, head) rows of D unnormalised sums, and (log2 max, sum)
   int B, n, h_q, h_kv, W, mask_lmk, expand, page_stride, num_pages, splits, row_blocks;
   float scale;
+  unsigned call;                       // number of the call, of the kernel with waits (tree_attn_tc.cu)
 };
 
 // Ancestors of the tree's nodes.  anc[j]: bits of j and its ancestors, 0 when j is absent: its parent is no earlier node

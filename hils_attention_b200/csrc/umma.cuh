@@ -11,7 +11,9 @@
 namespace hils {
 namespace umma {
 
-constexpr int kWaitPolls = 1 << 24;  // bounded mbarrier wait (well under a second of polling)
+// Bounded mbarrier wait.  The limit counts polls, not time: a poll may be held for a time that the hardware chooses, and a launch
+// whose waits ran out one after another has taken minutes with it.
+constexpr int kWaitPolls = 1 << 24;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 

@@ -436,3 +436,28 @@ def test_non_finite_cache_at_the_edge_of_the_window(hb, dtype, D, W, T, expand, 
     o[..., col] = ref[0][..., col].to(o)
     _near((o, lse), ref, dtype)
     assert _status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_captured_calls_replayed_in_turn_and_at_once(hb, dtype):
+    """Two captured calls of different shapes, replayed one after the other and side by side: each has a graph and scratch of its own."""
+    ps = [_problem(2, 12, 4, 2, 64, dtype, [3000, 200], ["random"], seed=4), _problem(3, 9, 8, 2, 128, dtype, [900, 70, 0], ["binary"], seed=5)]
+    alone, graphs, streams = [_call(hb, p) for p in ps], [], [torch.cuda.Stream() for _ in ps]
+    for p in ps:
+        args = [p["q"], p["k"], p["v"], p["kp"], p["vp"], p["table"].cuda(), p["lens"].cuda(), max(p["lens"].tolist()), p["parents"].cuda()]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = hb.tree_attn_paged(*args)
+        graphs.append((graph, out, args))
+    for side_by_side in (False, True):
+        for _ in range(10):
+            for graph, out, _ in graphs:
+                out[0].fill_(NAN), out[1].fill_(NAN)
+            torch.cuda.synchronize()
+            for (graph, _, _), s in zip(graphs, streams if side_by_side else [torch.cuda.current_stream()] * 2):
+                with torch.cuda.stream(s):
+                    graph.replay()
+            torch.cuda.synchronize()
+            for (_, out, _), ref in zip(graphs, alone):
+                assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
+    assert _status() == 0
