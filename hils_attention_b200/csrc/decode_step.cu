@@ -68,6 +68,7 @@ int topk_decode_step_launch(const void* q, const void* lmks, const void* lse_swa
                             int dtype, int lse_dtype, void* workspace, size_t workspace_bytes, cudaStream_t st);
 
 // tree_attn.cu, decode_attn.cu, topk.cu: the stages over drafted rows
+void tree_positions_launch(const int32_t* parents, const int32_t* lens, int32_t* positions, int B, int n, int max_len, cudaStream_t st);
 size_t tree_attn_workspace(int B, int n, int h_q, int h_kv, int D, int max_len, int W, int dtype);
 int tree_attn_launch(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages, const int32_t* page_table,
                      int page_stride, int num_pages, const int32_t* lens, int max_len, const int32_t* parents, void* o, float* lse,
@@ -243,7 +244,8 @@ extern "C" int hils_decode_tree_paged(const void* q, const void* lmk_q, const vo
   int32_t* positions = reinterpret_cast<int32_t*>(ws + lay.positions);
   int32_t* indices = indices_out ? indices_out : reinterpret_cast<int32_t*>(ws + lay.s.indices);
   // 1. positions of the nodes
-  if (int rc = hils_draft_positions(parents, lens, positions, B, n, stream)) return rc;
+  tree_positions_launch(parents, lens, positions, B, n, max_len, st);
+  HILS_LAUNCH_CHECK("decode_tree_paged (positions)");
   // 2. sliding-window branch: cached tokens of the window, ancestors, the node itself
   if (int rc = tree_attn_launch(q, k_new, v_new, k_pages, v_pages, page_table, page_stride, num_pages, lens, max_len, parents, swa_o,
                                 reinterpret_cast<float*>(ws + lay.s.lse32), lse_act, B, n, h_q, h_kv, D, window_size, 1, 1, sm_scale, dtype,

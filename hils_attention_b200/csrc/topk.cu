@@ -50,8 +50,9 @@ __device__ __forceinline__ int row_limit_b(const TopkParams& p, int b, int l) {
   if (!p.q_offsets && !p.row_pos) return row_limit(p, l);
   if (l >= p.L) return 0;
   if (!p.is_causal) return p.N;
-  const int t = p.row_pos ? p.row_pos[(int64_t)b * p.L + l] : p.q_offsets[b] + l;
+  int t = p.row_pos ? p.row_pos[(int64_t)b * p.L + l] : p.q_offsets[b] + l;
   if (p.row_pos && t < 0) return 0;
+  if (p.dots) t = min(t, p.q_offset + p.L - 1);           // the keys are streamed up to the host's bound: nothing is written behind it
   const int lim = (p.window_size > 0) ? floor_div(t - p.window_size + 1, p.block_size) : floor_div(t, p.block_size);
   return max(0, min(lim, p.N));
 }

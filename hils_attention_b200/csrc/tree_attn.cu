@@ -11,7 +11,8 @@
 
 namespace hils {
 
-// Set when a page table holds an id outside the pool or a sequence reaches past the table's width; the tile is skipped.
+// Set when a page table holds an id outside the pool (8200001; the tile is skipped), a sequence reaches past the table's width
+// (8200002; it is cut) or past the bound of a decode step (8200003).
 static __device__ int g_tree_status = 0;
 
 constexpr int kTreeThreads = 256, kTreeRows = 32;
@@ -259,12 +260,13 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
   }
 }
 
-// Positions of the nodes, -1 for those that are absent.
-__global__ void __launch_bounds__(kTreeMaxNodes) tree_positions_kernel(const int32_t* parents, const int32_t* lens, int32_t* pos, int n) {
+// Positions of the nodes, -1 for those that are absent.  A length past max_len is reported.
+__global__ void __launch_bounds__(kTreeMaxNodes) tree_positions_kernel(const int32_t* parents, const int32_t* lens, int32_t* pos, int n, int max_len) {
   __shared__ int par_s[kTreeMaxNodes];
   __shared__ u64t anc[kTreeMaxNodes + 1];
   const int b = blockIdx.x, j = threadIdx.x;
   tree_ancestors(tree_parents(parents + (int64_t)b * n, n, j), n, 0, 0, par_s, anc, j, 0, kTreeMaxNodes);
+  if (j == 0 && lens[b] > max_len) atomicExch(&g_tree_status, 8200003);
   if (j < n) pos[(int64_t)b * n + j] = anc[j] ? max(lens[b], 0) + __popcll(anc[j]) - 1 : -1;
 }
 
@@ -336,6 +338,10 @@ size_t tree_attn_workspace(int B, int n, int h_q, int h_kv, int D, int max_len, 
   return tree_workspace(tree_plan(B, n, h_q, h_kv, max_len, W, dtype), D);
 }
 
+void tree_positions_launch(const int32_t* parents, const int32_t* lens, int32_t* positions, int B, int n, int max_len, cudaStream_t st) {
+  tree_positions_kernel<<<(unsigned)B, kTreeMaxNodes, 0, st>>>(parents, lens, positions, n, max_len);
+}
+
 // Checked arguments; lse_act as in TreeParams.
 int tree_attn_launch(const void* q, const void* k_new, const void* v_new, const void* k_pages, const void* v_pages, const int32_t* page_table,
                      int page_stride, int num_pages, const int32_t* lens, int max_len, const int32_t* parents, void* o, float* lse,
@@ -401,7 +407,7 @@ extern "C" int hils_draft_positions(const int32_t* parents, const int32_t* lens,
   HILS_REQUIRE(B >= 0 && n >= 0 && n <= kTreeMaxNodes, "draft_positions: %d sequences of %d nodes (at most %d)", B, n, kTreeMaxNodes);
   if (B == 0 || n == 0) return HILS_OK;
   HILS_REQUIRE(parents && lens && positions, "draft_positions: null pointer");
-  tree_positions_kernel<<<(unsigned)B, kTreeMaxNodes, 0, (cudaStream_t)stream>>>(parents, lens, positions, n);
+  hils::tree_positions_launch(parents, lens, positions, B, n, 0x7fffffff, (cudaStream_t)stream);
   HILS_LAUNCH_CHECK("draft_positions");
   return HILS_OK;
 }

@@ -588,7 +588,7 @@ def decode_tree_paged(q, lmk_q, k_new, v_new, k_pages, v_pages, page_table, lens
 
     q, lmk_q (B, n, h_q, D), k_new, v_new (B, n, h_kv, D), parents (B, n) int32 as in `tree_attn_paged` (the window branch);
     every node selects its chunks and attends to them at its own position.  n <= 64 and n <= window_size.  The pages and
-    lens are left as they are: `commit_drafts` writes the accepted nodes.
+    lens are left as they are: `commit_drafts` writes the accepted nodes.  A captured step holds for lengths up to its max_len.
     Returns o (B, n, h_q, D) (zeros for absent nodes) [, indices (B, n, h_kv, topk)] and the workspace for reuse."""
     if q.dim() != 4 or lmk_q.shape != q.shape or k_new.dim() != 4 or k_new.shape != v_new.shape or k_new.shape[:2] != q.shape[:2]:
         raise ValueError(f"decode_tree_paged: q, lmk_q (B,n,h_q,D), k_new, v_new (B,n,h_kv,D), got {tuple(q.shape)}, {tuple(lmk_q.shape)}, "

@@ -394,7 +394,9 @@ int hils_draft_positions(const int32_t* parents, const int32_t* lens, int32_t* p
 /* hils_decode_tree_paged: the decode step of hils_decode_step_paged for a tree of drafted tokens per sequence (the tree
  *   attention as the window branch, selection and sparse chunk attention for every node at its own position).  Arguments as
  *   there with q, lmk_q, o (B, n, h_q, D), k_new, v_new (B, n, h_kv, D), parents (B, n), indices_out (B, n, h_kv, K) or
- *   NULL; the pages are only read; n <= window_size; lens is not advanced.  Absent nodes give o = 0. */
+ *   NULL; the pages are only read; n <= window_size; lens is not advanced.  Absent nodes give o = 0.  A captured step holds
+ *   for lengths up to the max_len of its capture; a longer one is reported through hils_take_device_status (8200003), and
+ *   chunks that the bound leaves out may not be selected. */
 int hils_decode_tree_paged(const void* q, const void* lmk_q, const void* k_new, const void* v_new, const void* k_pages,
                            const void* v_pages, const int32_t* page_table, int page_stride, int num_pages,
                            const int32_t* lens, int max_len, const int32_t* parents, const void* lmk_k,

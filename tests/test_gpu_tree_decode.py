@@ -276,3 +276,33 @@ def test_a_captured_step_replays_at_lengths_its_capture_did_not_have():
                     assert int(idx.max()) >= 1024
             store.release(1)
     assert _status() == 0
+
+
+def test_a_length_past_the_bound_is_reported_and_selects_from_written_scores_only():
+    """What a graph does whose sequence has outgrown the bound of its capture: the scores behind the bound are not computed."""
+    from hils_attention_b200 import ops
+    hq, hk, D, n, N, T, bound = 4, 2, 64, 3, 1200, 70000, 1000
+    g = torch.Generator(device="cuda").manual_seed(6)
+    mk = lambda *s: torch.randn(*s, generator=g, device="cuda").to(BF)
+    kp, vp, lmk = mk(1100, hk, 64, D), mk(1100, hk, 64, D), mk(1, N, hq, D)
+    table = torch.zeros(1, N, dtype=torch.int32, device="cuda")
+    table[0, :1099] = torch.arange(1, 1100, dtype=torch.int32)
+    lens = torch.tensor([T], dtype=torch.int32, device="cuda")
+    q, l, k, v = mk(1, n, hq, D), mk(1, n, hq, D), mk(1, n, hk, D), mk(1, n, hk, D)
+    parents = torch.tensor([[-1, 0, 1]], dtype=torch.int32, device="cuda")
+    call = lambda max_len, ws=None: ops.decode_tree_paged(q, l, k, v, kp, vp, table, lens, max_len, parents, lmk, None, K, 64, W, workspace=ws, return_indices=True)
+    full, ids, ws = call(T)
+    assert int(ids.max()) > bound // 64 and _status() == 0
+    for fill in (0x50, 0xd0, 0xff):                            # large scores, small ones, NaN
+        ws.fill_(fill)
+        o, ids, again = call(bound, ws)
+        assert again is ws and _status() == 8200003
+        assert int(ids.min()) >= 0 and int(ids.max()) < (bound + n - 1 - W + 1) // 64
+        assert bool(torch.isfinite(o).all())
+    for fill in (0x50, 0xff):                                  # the single-token step reads the same scores
+        one = torch.full((ws.numel(),), fill, dtype=torch.uint8, device="cuda")
+        _, ids, again = ops.decode_step_paged(q[:, 0].contiguous(), l[:, 0].contiguous(), k[:, 0].contiguous(), v[:, 0].contiguous(), kp, vp, table, lens, bound,
+                                              lmk, None, K, 64, W, workspace=one, return_indices=True)
+        assert again is one and int(ids.min()) >= 0 and int(ids.max()) < (bound - W + 1) // 64
+    o, ids, _ = call(T, ws)
+    assert torch.equal(o, full) and _status() == 0
