@@ -120,6 +120,7 @@ def dtype_code(t: torch.Tensor) -> int:
         return BF16
     if t.dtype == torch.float32:
         return F32
+    _pending().clear()                                         # no call follows: its tensors' devices are not the next call's
     raise TypeError(f"hils_b200 kernels take bfloat16 or float32 tensors, got {t.dtype}")
 
 
