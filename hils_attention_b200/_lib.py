@@ -216,12 +216,12 @@ def call(name: str, *args):
             rc = getattr(lib, name)(*args)
     else:
         rc = getattr(lib, name)(*args)
-    _launches += KERNELS_PER_CALL.get(name, 1)
     if rc != 0:
         msg = lib.hils_last_error().decode("utf-8", "replace")
         err = HilsError(f"{name} failed with status {rc}: {msg}")
         err.status = rc
         raise err
+    _launches += KERNELS_PER_CALL.get(name, 1)
     if _CHECK_STATUS:
         st = int(lib.hils_take_device_status())
         if st != 0:

@@ -12,3 +12,12 @@ def test_a_refused_type_leaves_no_devices_behind():
         with pytest.raises(TypeError):
             _lib.dtype_code(t)
         assert _lib._pending() == []
+
+
+def test_a_refused_call_is_not_counted_as_launched():
+    before = _lib.launch_count()
+    with pytest.raises(_lib.HilsError) as e:
+        _lib.call("hils_draft_positions", None, None, None, 1, 65, None)
+    assert e.value.status == -1 and _lib.launch_count() == before
+    _lib.call("hils_draft_positions", None, None, None, 0, 4, None)
+    assert _lib.launch_count() == before + 1
