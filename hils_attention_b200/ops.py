@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import functools
 import math
+import operator
 import struct
 from typing import Optional, Tuple
 
@@ -649,7 +650,11 @@ def _host_ids(x, what: str) -> torch.Tensor:
         if t.dim() != 1:
             raise ValueError(f"{what} must be one-dimensional, got shape {tuple(x.shape)}")
         return t.contiguous()
-    return torch.tensor(list(x), dtype=torch.int32)
+    ids = list(map(operator.index, x))                         # a float is no id
+    try:
+        return torch.tensor(ids, dtype=torch.int32)
+    except (OverflowError, RuntimeError):
+        raise ValueError(f"{what} do not fit 32 bits") from None
 
 
 def _pool_layers(k_pages, v_pages, what: str):

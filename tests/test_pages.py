@@ -215,3 +215,16 @@ def test_commit_drafts_checks_shapes_and_types():
             ops.commit_drafts(**{**ok, **change})
     with pytest.raises(RuntimeError):
         ops.commit_drafts(**ok)                 # not on a GPU
+
+
+def test_copy_pages_does_not_round_or_cut_page_ids():
+    k = torch.zeros(2, 8, 2, 64, 8)
+    for src, err in (([1.7], TypeError), ([1, 2.5], TypeError), ([2 ** 32 + 1], ValueError), ([-2 ** 31 - 1], ValueError), ([2 ** 70], ValueError), ([[1]], TypeError)):
+        with pytest.raises(err):
+            ops.copy_pages(k, k, src, [2] * len(src))
+        with pytest.raises(err):
+            ops.copy_pages(k, k, [2] * len(src), src)
+    for none in ([], (), range(0), torch.empty(0, dtype=torch.int64)):
+        ops.copy_pages(k, k, none, [])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.copy_pages(k, k, range(1, 3), (3, 4))
