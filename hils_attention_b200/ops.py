@@ -659,17 +659,20 @@ def _host_ids(x, what: str) -> torch.Tensor:
 
 def _pool_layers(k_pages, v_pages, what: str):
     """(layers, pages per layer, bytes from layer to layer) of two pools (num_layers, num_pages, h_kv, S, D) or one layer of them."""
-    shape, stride = k_pages.shape, k_pages.stride()
-    if shape != v_pages.shape or k_pages.dtype != v_pages.dtype or stride != v_pages.stride():
-        raise ValueError(f"{what}: k_pages and v_pages differ in shape, type or strides")
+    shape = k_pages.shape
+    if shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError(f"{what}: k_pages and v_pages differ in shape or type")
     if len(shape) not in (4, 5):
         raise ValueError(f"{what}: pools are (num_pages, h_kv, S, D) or (num_layers, num_pages, h_kv, S, D), got {tuple(shape)}")
-    pages, h, S, D = shape[-4:]
-    if pages * h * S * D and stride[-4:] != (h * S * D, S * D, D, 1):
-        raise ValueError(f"{what}: a layer's pool must be contiguous")
-    if len(shape) == 4:
-        return 1, pages, pages * h * S * D * k_pages.element_size()
-    return shape[0], pages, stride[0] * k_pages.element_size()
+    layers, pages = (1 if len(shape) == 4 else shape[0]), shape[-4]
+    page = shape[-3] * shape[-2] * shape[-1]
+    apart = k_pages.stride(0) if layers > 1 else pages * page
+    if layers > 1 and v_pages.stride(0) != apart:
+        raise ValueError(f"{what}: the layers of k_pages and v_pages are not the same way apart")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):         # some layers of a larger pool
+        if len(shape) == 4 or not (k_pages[0].is_contiguous() and v_pages[0].is_contiguous()):
+            raise ValueError(f"{what}: a layer's pool must be contiguous")
+    return layers, pages, apart * k_pages.element_size()
 
 
 def copy_pages(k_pages, v_pages, src, dst) -> None:

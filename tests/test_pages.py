@@ -228,3 +228,23 @@ def test_copy_pages_does_not_round_or_cut_page_ids():
         ops.copy_pages(k, k, none, [])
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.copy_pages(k, k, range(1, 3), (3, 4))
+
+
+def test_strides_of_dimensions_of_one_do_not_matter():
+    """One head, one page, one layer: a view that is contiguous with other strides there is a pool like any other."""
+    head = torch.zeros(3, 64, 1, 8).transpose(1, 2)                            # (3, 1, 64, 8)
+    page = torch.zeros(2, 1, 2, 64, 8).as_strided((2, 1, 2, 64, 8), (1024, 7, 512, 8, 1))
+    layer = torch.zeros(1, 3, 2, 64, 8).as_strided((1, 3, 2, 64, 8), (5, 1024, 512, 8, 1))
+    for k in (head, page, layer):
+        assert k.is_contiguous()
+        v = torch.zeros(k.shape)
+        if k.shape[-4] > 1:
+            for pools in ((k, v), (v, k)):
+                with pytest.raises(RuntimeError, match="CUDA"):                # past the checks
+                    ops.copy_pages(*pools, [1], [2])
+        assert ops._pool_layers(k, v, "pools") == ops._pool_layers(v, k, "pools") == ops._pool_layers(v, v, "pools")
+    some = torch.zeros(4, 3, 2, 64, 8)[::2]
+    assert ops._pool_layers(some, some, "pools") == (2, 3, 2 * 3 * 1024 * 4)
+    for k, v in ((some, torch.zeros(2, 3, 2, 64, 8)), (torch.zeros(2, 3, 64, 2, 8).transpose(2, 3),) * 2, (torch.zeros(3, 64, 2, 8).transpose(1, 2),) * 2):
+        with pytest.raises(ValueError):
+            ops.copy_pages(k, v, [1], [2])
