@@ -25,7 +25,7 @@ using namespace umma;
 
 static __device__ int g_cm_status = 0;
 
-// Bounded wait of this file's kernels: 2^20 polls (tens of milliseconds; a healthy wait lasts microseconds).
+// Bounded wait of this file's kernels: 2^20 polls (4 s; a healthy wait lasts microseconds).
 // After the first expiry anywhere on the device the status word is set and every CTA that starts later returns
 // at once, so a fault costs one wait, not one per CTA.
 __device__ __forceinline__ bool cm_wait(uint64_t* b, uint32_t parity) {

@@ -22,8 +22,9 @@
 // 256 rows in one CTA, which brings a tile once, took 179 (171 with one group at that time); P through shared memory 224.
 // Few rows: 16 nodes, 32 sequences x 32 heads, window 512: 83 us, floor 46 (302 MB).  While tiles run, 2 CTAs an SM ask for all
 // the HBM gives; of a CTA's 31000 clocks 5900 pass before its first tile and 4700 after its last, and 1024 CTAs are 3.46 waves.
-// Not faster for these: warp-level products, a persistent kernel, keys as the rows of the product (four CTAs an SM), rows dealt
-// to other warps.  Long caches with few rows run at 0.87 of the copy bandwidth (8 x 16000 tokens, 8 key heads: 92 us in a loop).
+// Not faster for these: keys as the rows of the product (four CTAs an SM: 92 us against 80 in the same loop), rows dealt to other
+// warps (D 64: 140 against 131).  Long caches with few rows run at 0.87 of the copy bandwidth (8 x 16000 tokens, 8 key heads: 92 us
+// in a loop).
 #include <algorithm>
 #include <atomic>
 
@@ -74,7 +75,7 @@ __device__ __forceinline__ bool not_finite8(uint4 x) {     // eight bf16: an exp
 // row `r` of a [64 x D] tile of DB column blocks, piece c of 16 bytes
 __device__ __forceinline__ uint8_t* tile_at(uint8_t* tile, int r, int c) { return tile + (c >> 3) * 8192 + sw128_off(r, c & 7); }
 
-// Fewer polls than the common limit: these waits are for copies and products of one tile, microseconds.
+// A second (2^18 polls of 3.95 us), shorter than the common limit: these waits are for copies and products of one tile, microseconds.
 __device__ __forceinline__ bool wait_for(uint64_t* b, uint32_t parity) { return mbar_wait<1 << 18>(b, parity); }
 
 // What the products left out for one row: the keys whose V rows were zeroed although this row sees them.  Rare (a value that
