@@ -4,7 +4,8 @@
 // plan of a call; bf16 runs tree_attn_tc.cu.  One CTA per (sequence, key head, 32 rows, share of the tiles).  K and V of a tile of
 // 64 keys go from registers, where they arrive while the tile before is computed, to shared memory; a thread forms 2 x 4 scores
 // and 2 x D/16 outputs; running maximum and sum per row.  What bounds it: latency at the sizes it is for.  9 nodes x 2 query heads
-// a key head, 2 sequences of 2003 tokens, D 64: 15.2 us and 8.2 for the join with cold caches (23 us a call in a loop).
+// a key head, 2 sequences of 2003 tokens, D 64: 15.2 us and 8.2 for the join with cold caches (23 us a call in a loop).  Where the
+// arithmetic binds (64 nodes x 4 a key head, 8 of them, 6000 tokens, D 128: 344 us) 18 TFLOP/s, held by shared-memory reads.
 #include <algorithm>
 
 #include "tree_common.cuh"

@@ -537,7 +537,7 @@ def tree_attn_paged(q, k_new, v_new, k_pages, v_pages, page_table, lens, max_len
     ancestor, makes the node absent (a shorter tree in a batch: pad with -2).  Node j stands at position lens[b] + depth; it
     sees the cached tokens, its ancestors and itself, within window_size positions (None: all; rounded down to whole chunks
     when expand_to_chunk), landmark positions excepted when mask_lmk, as flex_attn_tl.  The pages are only read: the
-    accepted tokens are written by commit_drafts.
+    accepted tokens are written by commit_drafts.  In bf16 the softmax weights are rounded to bf16 before they meet the values.
     Returns o (B, n, h_q, D), lse (B, n, h_q) fp32 (0 and -inf for rows that see nothing) and the workspace for reuse."""
     if q.dim() != 4 or k_new.dim() != 4:
         raise ValueError(f"tree_attn_paged: q (B,n,h_q,D), k_new and v_new (B,n,h_kv,D), got {tuple(q.shape)}, {tuple(k_new.shape)}")

@@ -378,7 +378,8 @@ size_t hils_qk_norm_rope_bwd_workspace_bytes(int D);
  *   Node j at position t = lens[b] + depth sees the cached tokens and, of the drafted ones, itself and its ancestors, from
  *   position t - window_size + 1 on (rounded down to its chunk when expand_to_chunk), without the landmark positions
  *   ((position + 1) % 64 == 0) when mask_lmk; a row that sees nothing gives o = 0, lse = -inf.  What lies in places no row
- *   sees (behind a sequence's last token, say) may be anything, NaN included.  D 64 or 128, sm_scale > 0.
+ *   sees (behind a sequence's last token, say) may be anything, NaN included.  D 64 or 128, sm_scale > 0.  bf16: the softmax
+ *   weights are rounded to bf16 before they meet the values; scores, sums and lse are fp32.
  *   workspace: hils_tree_attn_paged_workspace_bytes() (0 when none is needed).  A page outside the pool or the table is
  *   skipped and reported through hils_take_device_status (8200001, 8200002).
  * hils_draft_positions: positions (B, n) int32 of the nodes, -1 for absent ones.
