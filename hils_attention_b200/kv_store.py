@@ -122,8 +122,9 @@ class PagedKVStore:
         self.h_lmk = int(h_lmk if h_lmk is not None else h_q)
         self.pool = PagePool(num_pages)
         dev = torch.device(device)
-        self.device, self.dtype = dev, dtype
+        self.dtype = dtype
         self.k_pages = torch.zeros((num_layers, num_pages, h_kv, self.S, head_dim), dtype=dtype, device=dev)
+        dev = self.device = self.k_pages.device                     # with its index: "cuda" alone means another device later
         self.v_pages = torch.zeros_like(self.k_pages)
         self.page_table = torch.zeros((max_seqs, max_pages_per_seq), dtype=torch.int32, device=dev)   # 0 = scratch page
         self.lens = torch.zeros((max_seqs,), dtype=torch.int32, device=dev)

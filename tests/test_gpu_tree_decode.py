@@ -306,3 +306,16 @@ def test_a_length_past_the_bound_is_reported_and_selects_from_written_scores_onl
         assert again is one and int(ids.min()) >= 0 and int(ids.max()) < (bound - W + 1) // 64
     o, ids, _ = call(T, ws)
     assert torch.equal(o, full) and _status() == 0
+
+
+def test_a_store_stays_on_its_device():
+    """A store made on "cuda" is on the device that was current then, and so is all it makes later."""
+    from hils_attention_b200.kv_store import PagedKVStore
+    store = PagedKVStore(8, 2, 4, 2, 64, 4, device="cuda")
+    assert store.device == store.k_pages.device and store.device.index is not None
+    store.allocate(10)
+    store.begin_tree(3)
+    assert all(t.device == store.device for t in store.draft(0))
+    store.accept_tree([[0]])
+    store.end_tree()
+    assert store.lens.tolist() == [11, 0]
